@@ -5,13 +5,13 @@
 // Why not the matrix cores here (round-3 profile, profiles/r03_layers_b8.csv): the 16-row MFMA tiles of spconv.hip run these
 // layers at 12-37 TFLOP/s and at a quarter of the HBM rate -- neither roof.  Their limiter is vector-memory ISSUE: per (16-row
 // group, tap) a wave spends an index load, a 16-row gather and a weight-fragment load (2.25-3 instructions) to feed two to four
-// MFMAs, half of whose output columns are padding at Cout = 8.  The fp32 VALU peak of the part equals its fp32 MFMA peak
-// (v_pk_fma_f32: 2 x 64 FMA per 4 cycles), so the contraction moves to the VALU and the memory side is rebuilt around it:
+// MFMAs, half of whose output columns are padding at Cout = 8.  So the contraction moves to the VALU and the memory side is rebuilt
+// around it:
 //
 //   * one lane = one output row (RPL rows per lane): per (64 rows, tap) ONE coalesced index load (256 B) and Cin/4 b128 gathers
 //     (a lane reads its neighbour's whole row) -- 3 vector-memory instructions per 64 rows and tap instead of 9-12;
 //   * the tap's weights are wave-uniform: they come through the SCALAR cache (s_load_dwordx16 from the constant address space)
-//     into SGPRs and enter v_pk_fma_f32 as the scalar operand; no weight fragments through the vector memory path at all, and
+//     into SGPRs and enter v_fma_f32 as the scalar operand; no weight fragments through the vector memory path at all, and
 //     no Cout 8 -> 16 padding (a lane holds exactly Cout accumulators);
 //   * taps are walked through the union of the tile's active-tap masks; a lane whose own 16-row group lacks the tap replaces the
 //     (possibly unwritten: sparse table stores) entry by -1, whose gather the buffer descriptor answers with zeros.
@@ -43,13 +43,10 @@ __device__ __forceinline__ int rl_pop_or_keep(uint64_t& lo, uint64_t& hi, int ke
     return any ? k : keep;
 }
 
-// acc(lo, hi) += x * (w.lo, w.hi) with x = the low (HI = 0) or high (HI = 1) half of the register pair `xp`, broadcast by op_sel;
-// w is an SGPR pair.  (Inline asm: from plain vector code hipcc broadcasts an odd element by copying it into the low half of a
-// fresh register pair first -- and hoists those copies to the end of the previous loop iteration, where they wait for the loads.)
-template <int HI>
-__device__ __forceinline__ void pk_fma_bcast(f32x2& acc, const f32x2 xp, const f32x2 w) {
-    if constexpr (HI) asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[1,0,0] op_sel_hi:[1,1,1]" : "+v"(acc) : "v"(xp), "s"(w));
-    else asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,0,0] op_sel_hi:[0,1,1]" : "+v"(acc) : "v"(xp), "s"(w));
+// acc(lo, hi) += x * (w.lo, w.hi); w is an SGPR pair (one v_fma_f32 each: the packed form is not used, see the compile flags)
+__device__ __forceinline__ void fma_bcast(f32x2& acc, const float x, const f32x2 w) {
+    acc[0] = __builtin_fmaf(x, w[0], acc[0]);
+    acc[1] = __builtin_fmaf(x, w[1], acc[1]);
 }
 
 // CIN in {8, 16}; CO in {8, 16} (== the layer's cout); RPL rows per lane
@@ -152,9 +149,7 @@ __global__ void __launch_bounds__(64) k_conv_rowlane(ConvP P) {
 #pragma unroll
                 for (int q = 0; q < RPL; ++q) {
                     const f32x4 xr = x[q][ci >> 2];
-                    const f32x2 xp = (ci & 2) ? (f32x2){xr[2], xr[3]} : (f32x2){xr[0], xr[1]};
-                    if (ci & 1) pk_fma_bcast<1>(acc[q][c], xp, w2);
-                    else pk_fma_bcast<0>(acc[q][c], xp, w2);
+                    fma_bcast(acc[q][c], xr[ci & 3], w2);
                 }
             }
         }
