@@ -812,6 +812,41 @@ int insmos_debug_table_limit(int64_t bytes); /* tests only: lower the table size
 int insmos_forward_windows(void* ctx, const float* const* points_host, const int64_t* n_points_host, int B, int ld_pts,
                            void* arena, size_t arena_bytes, void* stream, InsmosForwardOut* outs);
 
+/* ------------------------------------------------------------------------------------------------
+ * The optimiser step over a list of tensors (models/models.py:185-190 trains with Adam): csrc/optim.hip.
+ *   g' = c g (+ weight_decay p if !decoupled);  m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2
+ *   p = p (1 - lr weight_decay if decoupled) - lr / (1 - b1^t) * (m / (sqrt(v) / sqrt(1 - b2^t) + eps))
+ * c = min(1, max_norm / (norm + 1e-6)) where max_norm > 0, else 1; norm = norm_in[0] if given, else that of the list's gradients.
+ * tensors_host: the list (HOST memory, read during the call only); dtype of all parameters and gradients: INSMOS_F32 / BF16 / F16.
+ * State buffers of n_state elements (a multiple of 256), 16-byte aligned; tensor i uses [state_off, state_off + numel) of them, the
+ * rest of its last 256 elements is kept zero.  state_bits 32: exp_avg = m, exp_avg_sq = v in fp32.  state_bits 8: e4m3 codes of m and
+ * of sqrt(v), in units of scales[0][n_state / 256] and scales[1][.] (fp32, largest of a block's 256 elements / 448), rounded
+ * stochastically by a hash of (element, step, seed).  masters: fp32 weights in the state layout that a BF16 / F16 list is updated
+ * from and rounded from, or NULL.  step: int32 counter of the steps done, advanced by the call.  lr_dev: fp32 learning rate in device
+ * memory, or NULL (then lr).  skip_nonfinite: a norm that is inf or NaN leaves everything as it was (the counter too).
+ * norm_out: receives the norm (fp32), or NULL.  No memory is kept between calls and nothing is read back: the calls can be captured.
+ * ---------------------------------------------------------------------------------------------- */
+#define INSMOS_F32 0
+#define INSMOS_BF16 1
+#define INSMOS_F16 2
+typedef struct InsmosOptTensor {
+    void* param;         /* (unused by the norm) */
+    const void* grad;
+    int64_t numel;
+    int64_t state_off;   /* start in the state buffers, a multiple of 256 */
+} InsmosOptTensor;
+/* The gradients' sum of squares as insmos_grad_sumsq_partials() fp64 partial sums (lists of several dtypes: one call each into one
+ * array), and the norm of everything in that array. */
+size_t insmos_grad_sumsq_partials(const InsmosOptTensor* tensors_host, int n_tensors);
+int insmos_grad_sumsq(const InsmosOptTensor* tensors_host, int n_tensors, int dtype, double* partials, int64_t n_partials,
+                      void* stream);
+int insmos_grad_norm(const double* partials, int64_t n_partials, float* norm, void* stream);
+size_t insmos_adamw_ws_bytes(const InsmosOptTensor* tensors_host, int n_tensors);
+int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dtype, int state_bits, void* exp_avg, void* exp_avg_sq,
+                      float* scales, int64_t n_state, float* masters, int32_t* step, double lr, const float* lr_dev, double beta1,
+                      double beta2, double eps, double weight_decay, int decoupled, double max_norm, const float* norm_in,
+                      int skip_nonfinite, unsigned seed, float* norm_out, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -176,6 +176,12 @@ SIGNATURES = {
     "insmos_center_head_loss_ws_floats": (c_sz, [c_i64, c_int]),
     "insmos_center_head_loss": (c_int, [c_vp, c_int, c_vp, c_int, c_i64, c_int, c_vp, c_vp, c_vp, c_vp, c_int, c_f32, c_f32,
                                         c_vp, c_vp, c_vp, c_int, c_vp, c_int, c_vp, c_vp]),
+    "insmos_grad_sumsq_partials": (c_sz, [c_vp, c_int]),
+    "insmos_grad_sumsq": (c_int, [c_vp, c_int, c_int, c_vp, c_i64, c_vp]),
+    "insmos_grad_norm": (c_int, [c_vp, c_i64, c_vp, c_vp]),
+    "insmos_adamw_ws_bytes": (c_sz, [c_vp, c_int]),
+    "insmos_adamw_step": (c_int, [c_vp, c_int, c_int, c_int, c_vp, c_vp, c_vp, c_i64, c_vp, c_vp, c_f64, c_vp, c_f64, c_f64, c_f64,
+                                  c_f64, c_int, c_f64, c_vp, c_int, c_u32, c_vp, c_vp, c_sz, c_vp]),
     "insmos_ctx_create": (c_int, [c_vp, c_vp, c_vp, c_int, c_vp]),
     "insmos_ctx_destroy": (c_int, [c_vp]),
     "insmos_forward_window": (c_int, [c_vp, c_vp, c_i64, c_int, c_vp, c_sz, c_vp, c_vp]),

@@ -1,0 +1,274 @@
+"""The optimiser step on MI355X: AdamW (or Adam with coupled weight decay, which models/models.py:185-190 trains with) over a whole
+list of tensors in one short chain of HIP launches (csrc/optim.hip), moments in 32 or in 8 bits, with the clip by the gradients'
+global norm inside the step.
+
+  * AdamW: a torch.optim.Optimizer (learning-rate schedulers, param_groups, state_dict work as usual).
+  * adamw_step(): the step itself on flat state buffers.
+  * grad_norm(): the global 2-norm of a list of gradients, on the device.
+
+State layout: the moments of a list (and its fp32 master weights) lie in one buffer each; tensor i starts at
+256 * sum_{j<i} ceil(numel_j / 256) (state_offsets()), in the tensor's own memory order, and what lies behind its end is zero.
+In 8 bits exp_avg holds e4m3 codes of m and exp_avg_sq those of sqrt(v), in units of scales[0] / scales[1], one fp32 value per 256
+elements; codes are rounded stochastically by a hash of (element, step, seed), so a step is reproducible.
+
+Nothing is read back from the device and no memory is kept between calls of the functions, so a step can be captured in a graph; a
+captured step repeats with the addresses of the tensors it was captured with and the learning rate it was captured with unless that
+is a tensor.
+"""
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+STATE_BLOCK = 256     # elements per scale; a tensor's start in the state buffers is a multiple of it
+_ENTRY = 32           # bytes of an InsmosOptTensor
+
+
+def state_offsets(sizes):
+    """Starts of tensors of these sizes in the state buffers, and the buffers' length."""
+    starts, at = [], 0
+    for n in sizes:
+        starts.append(at)
+        at += -(-int(n) // STATE_BLOCK) * STATE_BLOCK
+    return starts, at
+
+
+def _table(what, params, grads):
+    """(table, its entries, dtype code, length of the state buffers, tensors that the table points into beside the caller's)"""
+    from . import _host
+    table, extra = bytearray(_ENTRY * max(1, len(grads))), None
+    used, dtype, total, reorder = _host.opt_table(what, params, grads, table, False)
+    if reorder:
+        extra = list(grads)
+        for i in reorder:      # gradients in their parameter's memory order (or, alone, any dense one)
+            p = grads[i] if params is None else params[i]
+            extra[i] = p.contiguous() if params is None else torch.empty_strided(p.shape, p.stride(), dtype=p.dtype,
+                                                                                 device=p.device).copy_(grads[i])
+        used, dtype, total, _ = _host.opt_table(what, params, extra, table, False)
+    return (ctypes.c_char * len(table)).from_buffer(table), used, dtype, total, extra
+
+
+def grad_norm(grads):
+    """The 2-norm over all elements of the tensors (None entries are left out) as a 0-dim float32 tensor on their device; several
+    dtypes may be mixed.  Summed in fp64, in a fixed order: the same gradients give the same bits."""
+    grads = [g for g in grads if g is not None]
+    if not grads:
+        raise ValueError("grad_norm: no gradients")
+    lib = _lib.load()
+    lists = {}
+    for g in grads:
+        lists.setdefault(g.dtype, []).append(g)
+    dev = grads[0].device
+    tables = [_table("grad_norm", None, ts) for ts in lists.values()]
+    if any(ts[0].device != dev for ts in lists.values()):
+        raise ValueError("grad_norm: all tensors on one device")
+    with torch.cuda.device(dev):
+        st = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+        counts = [int(lib.insmos_grad_sumsq_partials(t[0], t[1])) for t in tables]
+        partials = torch.empty(max(1, sum(counts)), dtype=torch.float64, device=dev)
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        at = 0
+        for (table, used, dtype, _, _extra), n in zip(tables, counts):
+            _lib.check(lib.insmos_grad_sumsq(table, used, dtype, partials.data_ptr() + 8 * at, n, st), "insmos_grad_sumsq")
+            at += n
+        _lib.check(lib.insmos_grad_norm(partials.data_ptr(), at, norm.data_ptr(), st), "insmos_grad_norm")
+    return norm
+
+
+def _flat(what, t, dtype, n, dev):
+    if t.dtype != dtype or t.device != dev or not t.is_contiguous() or t.numel() != n:
+        raise ValueError(f"adamw_step: {what} is a contiguous {dtype} tensor of {n} elements on {dev}, "
+                         f"not {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.data_ptr() % 16:
+        raise ValueError(f"adamw_step: {what} starts on a 16-byte boundary")
+
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, decoupled=True,
+               scales=None, masters=None, max_grad_norm=None, grad_norm=None, skip_nonfinite=False, seed=0):
+    """One step over `params` (in place) with `grads` (None entries: that tensor and its state stay as they are).
+
+    params, grads: lists of the same length, float32, bfloat16 or float16 (one dtype and device), dense in memory; a parameter may
+      appear once.  exp_avg, exp_avg_sq: the moments in the state layout above, both float32, or both torch.float8_e4m3fn with
+      scales = float32 (2, length / 256).  step: int32 tensor of one element, the steps done so far; it is advanced.
+    lr: a number, or a float32 tensor of one element on the device.  decoupled: AdamW; False: the decay is added to the gradient.
+    masters: float32 weights in the state layout (bfloat16 / float16 params only): they are updated, params become their rounding.
+    max_grad_norm: the gradients count as scaled by min(1, max_grad_norm / (norm + 1e-6)); they are not changed.
+    grad_norm: the norm to clip by, a float32 tensor of one element (grad_norm() of more than this list); None: this list's.
+    skip_nonfinite: where the norm is inf or NaN nothing changes, the counter neither.
+    Returns the norm as a 0-dim float32 tensor where it was taken or given, else None."""
+    params, grads = list(params), list(grads)
+    b1, b2 = (float(b) for b in betas)
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+        raise ValueError(f"adamw_step: betas in [0, 1), not {tuple(betas)}")
+    eps, weight_decay = float(eps), float(weight_decay)
+    if not 0.0 <= eps < math.inf or not 0.0 <= weight_decay < math.inf:
+        raise ValueError(f"adamw_step: eps and weight_decay at least 0, not {eps}, {weight_decay}")
+    if max_grad_norm is not None and not float(max_grad_norm) > 0.0:
+        raise ValueError(f"adamw_step: max_grad_norm above 0 or None, not {max_grad_norm}")
+    table, used, dtype, total, _extra = _table("adamw_step", params, grads)
+    dev = params[0].device
+    bits = 8 if exp_avg.dtype == torch.float8_e4m3fn else 32
+    state = torch.float8_e4m3fn if bits == 8 else torch.float32
+    _flat("exp_avg", exp_avg, state, total, dev)
+    _flat("exp_avg_sq", exp_avg_sq, state, total, dev)
+    if bits == 8:
+        if scales is None:
+            raise ValueError("adamw_step: moments in 8 bits need scales")
+        _flat("scales", scales, torch.float32, 2 * total // STATE_BLOCK, dev)
+    elif scales is not None:
+        raise ValueError("adamw_step: scales belong to moments in 8 bits")
+    if masters is not None:
+        if dtype == 0:
+            raise ValueError("adamw_step: masters belong to bfloat16 or float16 parameters")
+        _flat("masters", masters, torch.float32, total, dev)
+    if step.dtype != torch.int32 or step.numel() != 1 or step.device != dev:
+        raise ValueError(f"adamw_step: step is one int32 on {dev}, not {step.dtype} {tuple(step.shape)} on {step.device}")
+    lr_dev = None
+    if torch.is_tensor(lr) and lr.device == dev:
+        if lr.dtype != torch.float32 or lr.numel() != 1:
+            raise ValueError(f"adamw_step: lr is a number or one float32, not {lr.dtype} {tuple(lr.shape)}")
+        lr_dev, lr_host = lr.data_ptr(), 0.0
+    else:
+        lr_host = float(lr)
+        if not 0.0 <= lr_host < math.inf:
+            raise ValueError(f"adamw_step: lr at least 0, not {lr_host}")
+    norm_in = None
+    if grad_norm is not None:
+        if grad_norm.dtype != torch.float32 or grad_norm.numel() != 1 or grad_norm.device != dev:
+            raise ValueError(f"adamw_step: grad_norm is one float32 on {dev}, not {grad_norm.dtype} on {grad_norm.device}")
+        norm_in = grad_norm.data_ptr()
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        norm_out = None
+        if grad_norm is None and (max_grad_norm is not None or skip_nonfinite):
+            norm_out = torch.empty((), dtype=torch.float32, device=dev)
+        need = int(lib.insmos_adamw_ws_bytes(table, used))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.check(lib.insmos_adamw_step(
+            table, used, dtype, bits, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+            scales.data_ptr() if scales is not None else None, total, masters.data_ptr() if masters is not None else None,
+            step.data_ptr(), lr_host, lr_dev, b1, b2, eps, weight_decay, 1 if decoupled else 0,
+            float(max_grad_norm) if max_grad_norm is not None else 0.0, norm_in, 1 if skip_nonfinite else 0, int(seed) & 0xFFFFFFFF,
+            norm_out.data_ptr() if norm_out is not None else None, ws.data_ptr(), need,
+            ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)), "insmos_adamw_step")
+    written = params if used == len(params) else [p for p, g in zip(params, grads) if g is not None]
+    torch.autograd.graph.increment_version(written + [exp_avg, exp_avg_sq, step] + [t for t in (scales, masters) if t is not None])
+    return grad_norm if grad_norm is not None else norm_out
+
+
+class _Bucket:
+    """The state of one group's parameters of one dtype and device."""
+
+    def __init__(self, params, state_bits, master_weights):
+        self.params = params
+        dev, dtype = params[0].device, params[0].dtype
+        self.starts, total = state_offsets([p.numel() for p in params])
+        state = torch.float8_e4m3fn if state_bits == 8 else torch.float32
+        self.exp_avg, self.exp_avg_sq = (torch.zeros(total, dtype=torch.float32, device=dev).to(state) for _ in range(2))
+        self.scales = torch.zeros((2, total // STATE_BLOCK), dtype=torch.float32, device=dev) if state_bits == 8 else None
+        self.step = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.masters = None
+        if master_weights and dtype != torch.float32:
+            self.masters = torch.zeros(total, dtype=torch.float32, device=dev)
+            for i in range(len(params)):
+                self.view(self.masters, i).copy_(params[i].detach())
+
+    def view(self, flat, i):
+        """Tensor i's part of a state buffer, shaped and ordered as the parameter."""
+        p = self.params[i]
+        return torch.as_strided(flat, p.shape, p.stride(), self.starts[i])
+
+    def entries(self, i):
+        """What a state_dict holds of parameter i (views of the buffers; the scales are the blocks' that the tensor covers)."""
+        out = {"step": self.step, "exp_avg": self.view(self.exp_avg, i), "exp_avg_sq": self.view(self.exp_avg_sq, i)}
+        if self.scales is not None:
+            a = self.starts[i] // STATE_BLOCK
+            out["scales"] = self.scales[:, a:a + -(-self.params[i].numel() // STATE_BLOCK)]
+        if self.masters is not None:
+            out["master"] = self.view(self.masters, i)
+        return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled=False: Adam with the decay in the gradient) whose step() is adamw_step() on every parameter group.
+
+    state_bits: 32, or 8 (4 bytes less than half a byte over 2 per parameter instead of 8).  master_weights: keep fp32 weights of
+    bfloat16 / float16 parameters.  max_grad_norm: clip by the norm over ALL gradients of the optimiser.  skip_nonfinite: a step whose
+    gradients' norm is inf or NaN changes nothing.  seed: of the 8-bit rounding.  lr may be a float32 tensor on the device (a captured
+    step then follows it).  After step(), last_grad_norm holds the norm (None where it was not taken).
+
+    A group's parameters share one step counter; a parameter without a gradient keeps its value and moments.  The state is made at the
+    first step (or load_state_dict) from the parameters as they are then, and a group's list is fixed from then on."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, decoupled=True, state_bits=32,
+                 master_weights=False, max_grad_norm=None, skip_nonfinite=False, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits is 8 or 32, not {state_bits}")
+        if not torch.is_tensor(lr) and not 0.0 <= float(lr) < math.inf:
+            raise ValueError(f"AdamW: lr at least 0, not {lr}")
+        if max_grad_norm is not None and not float(max_grad_norm) > 0.0:
+            raise ValueError(f"AdamW: max_grad_norm above 0 or None, not {max_grad_norm}")
+        self.state_bits, self.master_weights = int(state_bits), bool(master_weights)
+        self.max_grad_norm, self.skip_nonfinite, self.seed = max_grad_norm, bool(skip_nonfinite), int(seed)
+        self.last_grad_norm = None
+        self._buckets = {}      # group index -> list of _Bucket
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled=decoupled))
+
+    def _group_buckets(self, gi):
+        if gi not in self._buckets:
+            lists = {}
+            for p in self.param_groups[gi]["params"]:
+                lists.setdefault((p.device, p.dtype), []).append(p)
+            self._buckets[gi] = [_Bucket(ps, self.state_bits, self.master_weights) for ps in lists.values()]
+            for b in self._buckets[gi]:
+                for i, p in enumerate(b.params):
+                    self.state[p] = b.entries(i)
+        return self._buckets[gi]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = []
+        for gi, group in enumerate(self.param_groups):
+            for b in self._group_buckets(gi):
+                grads = [p.grad for p in b.params]
+                if any(g is not None for g in grads):
+                    work.append((group, b, grads))
+        norm = None
+        wanted = self.max_grad_norm is not None or self.skip_nonfinite
+        if wanted and len(work) > 1:
+            norm = grad_norm([g for _, _, grads in work for g in grads])
+        for group, b, grads in work:
+            norm_b = adamw_step(b.params, grads, b.exp_avg, b.exp_avg_sq, b.step, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                                weight_decay=group["weight_decay"], decoupled=group["decoupled"], scales=b.scales, masters=b.masters,
+                                max_grad_norm=self.max_grad_norm, grad_norm=norm, skip_nonfinite=self.skip_nonfinite, seed=self.seed)
+        self.last_grad_norm = norm_b if work and wanted else None
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """A state_dict() of an AdamW with the same state_bits and master_weights over parameters of the same shapes."""
+        state = state_dict["state"]
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        self._buckets.clear()
+        self.state.clear()
+        at = 0
+        for gi, group in enumerate(self.param_groups):
+            index = {id(p): at + i for i, p in enumerate(group["params"])}
+            at += len(index)
+            if not any(j in state for j in index.values()):
+                continue
+            for b in self._group_buckets(gi):
+                for i, p in enumerate(b.params):
+                    got, have = state.get(index[id(p)]), b.entries(i)
+                    if got is None:
+                        continue
+                    if set(got) != set(have) or any(got[k].shape != have[k].shape or got[k].dtype != have[k].dtype for k in have):
+                        raise ValueError(f"AdamW.load_state_dict: the state of parameter {index[id(p)]} is of another kind or shape "
+                                         f"(state_bits {self.state_bits}, master_weights {self.master_weights} here)")
+                    for k in have:
+                        have[k].copy_(got[k])
