@@ -26,14 +26,14 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-template <class T> struct Vec;
-template <> struct Vec<float> { typedef f32x4 t; };
-template <> struct Vec<__bf16> { typedef bf16x4 t; };
-template <> struct Vec<_Float16> { typedef f16x4 t; };
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+// eight values in memory at the alignment of one (the hardware takes 16-byte accesses at any address)
+template <class T> struct Mem8;
+template <> struct Mem8<float> { typedef float t __attribute__((ext_vector_type(8), aligned(4))); };
+template <> struct Mem8<__bf16> { typedef __bf16 t __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct Mem8<_Float16> { typedef _Float16 t __attribute__((ext_vector_type(8), aligned(2))); };
 
 enum { KC = 0, NC = 1 };                                            // which index of an operand is contiguous
 enum { T256 = 0, T128 = 1, TNARROW = 2, TFLAT = 3 };                // tiles 256x256, 128x128, 128x32 (few columns), 32x128 (few rows)
@@ -55,21 +55,19 @@ struct GemmP {
     void* z;              // the value before the activation, or null
     int64_t ld_z;
     int act, res_first;
-    int vec;              // y, z, res, bias allow accesses of 4 values
 };
 
 // ---- activations ------------------------------------------------------------------------------------------------------------
 // (v_exp and v_rcp: 1 ulp each; exp(-x) = inf gives 0)
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 constexpr float kGelu0 = 0.7978845608028654f, kGelu1 = 0.044715f;   // sqrt(2 / pi) (z + 0.044715 z^3)
+// act != INSMOS_ACT_NONE.  z times a weight between 0 and 1; silu's and the tanh form's are sigmoids: (1 + tanh u) / 2 = sigmoid(2 u).  (One formula for both: the
+// epilogue's code is part of every tile's time when it has to be fetched.)
 __device__ __forceinline__ float activate(float z, int act) {
-    switch (act) {
-        case INSMOS_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
-        case INSMOS_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.7071067811865476f));
-        case INSMOS_ACT_GELU_TANH: return z * sigmoid(2.f * kGelu0 * (z + kGelu1 * z * z * z));   // (1 + tanh u) / 2 = sigmoid(2 u)
-        case INSMOS_ACT_SILU: return z * sigmoid(z);
-    }
-    return z;
+    if (act == INSMOS_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+    if (act == INSMOS_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.7071067811865476f));
+    const float c0 = act == INSMOS_ACT_SILU ? 1.f : 2.f * kGelu0, c1 = act == INSMOS_ACT_SILU ? 0.f : 2.f * kGelu0 * kGelu1;
+    return z * sigmoid(z * (c0 + c1 * (z * z)));
 }
 __device__ __forceinline__ float slope(float z, int act) {
     switch (act) {
@@ -83,40 +81,47 @@ __device__ __forceinline__ float slope(float z, int act) {
     }
     return 1.f;
 }
-// values n..n+3 of row m, from the fp32 sums
 template <class T>
-__device__ __forceinline__ void epilogue(const GemmP& p, int m, int n, f32x4 v) {
-    typedef typename Vec<T>::t T4;
-    const T* bias = (const T*)p.bias;
-    const T* res = p.res ? (const T*)p.res + (int64_t)m * p.ld_res : nullptr;
-    T* y = (T*)p.y + (int64_t)m * p.ld_y;
-    T* z = p.z ? (T*)p.z + (int64_t)m * p.ld_z : nullptr;
-    if (p.vec && n + 4 <= p.N) {
-        if (bias) v += __builtin_convertvector(*(const T4*)(bias + n), f32x4);
-        f32x4 r = {0.f, 0.f, 0.f, 0.f};
-        if (res) r = __builtin_convertvector(*(const T4*)(res + n), f32x4);
-        if (p.res_first) v += r;
-        if (z) *(T4*)(z + n) = __builtin_convertvector(v, T4);
-        if (p.act) {
+__device__ __forceinline__ f32x8 load8(const void* q, int64_t i) { return __builtin_convertvector(*(const typename Mem8<T>::t*)((const T*)q + i), f32x8); }
+template <class T>
+__device__ __forceinline__ void store8(void* q, int64_t i, f32x8 v) {
+    typedef typename Mem8<T>::t M8;
+    *(M8*)((T*)q + i) = __builtin_convertvector(v, M8);
+}
+// values n..n+7 of row m from the fp32 sums, all inside the matrix; b and r: bias and residual (zeros where there is none)
+template <class T>
+__device__ __forceinline__ void epilogue8(const GemmP& p, int m, int n, f32x8 v, f32x8 b, f32x8 r) {
+    v += b;
+    if (p.res_first) v += r;
+    if (p.z) store8<T>(p.z, m * p.ld_z + n, v);
+    if (p.act) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = activate(v[e], p.act);
-        }
-        if (res && !p.res_first) v += r;
-        *(T4*)(y + n) = __builtin_convertvector(v, T4);
-        return;
+        for (int e = 0; e < 8; ++e) v[e] = activate(v[e], p.act);
     }
+    if (!p.res_first) v += r;
+    store8<T>(p.y, m * p.ld_y + n, v);
+}
+// the same one by one, up to the matrix's edge
+template <class T>
+__device__ __forceinline__ void epilogue1(const GemmP& p, int m, int n, f32x8 v) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 8; ++e) {
         if (n + e >= p.N) break;
         float u = v[e];
-        if (bias) u += (float)bias[n + e];
-        const float r = res ? (float)res[n + e] : 0.f;
+        if (p.bias) u += (float)((const T*)p.bias)[n + e];
+        const float r = p.res ? (float)((const T*)p.res)[m * p.ld_res + n + e] : 0.f;
         if (p.res_first) u += r;
-        if (z) z[n + e] = (T)u;
-        u = activate(u, p.act);
-        if (res && !p.res_first) u += r;
-        y[n + e] = (T)u;
+        if (p.z) ((T*)p.z)[m * p.ld_z + n + e] = (T)u;
+        if (p.act) u = activate(u, p.act);
+        if (!p.res_first) u += r;
+        ((T*)p.y)[m * p.ld_y + n + e] = (T)u;
     }
+}
+template <class T>
+__device__ __forceinline__ void epilogue(const GemmP& p, int m, int n, f32x8 v) {
+    if (n + 8 > p.N) return epilogue1<T>(p, m, n, v);
+    const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    epilogue8<T>(p, m, n, v, p.bias ? load8<T>(p.bias, n) : zero, p.res ? load8<T>(p.res, m * p.ld_res + n) : zero);
 }
 
 // ---- operands ---------------------------------------------------------------------------------------------------------------
@@ -240,6 +245,8 @@ template <> __device__ __forceinline__ f32x16 mfma<float>(f32x4 b, f32x4 a, f32x
 }
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------------
+struct Item { int tm, tn, split, kt0, kt1; };   // a tile of C and a part of k
+
 template <class T, int LA, int LB, int BM, int BN, int WM, int WN>
 struct Gemm {
     static constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32, SA = BM * 128, SB = BN * 128, BK = 128 / sizeof(T);
@@ -248,47 +255,109 @@ struct Gemm {
     typedef Frag<T, LA, BM, TM> FA;
     typedef Frag<T, LB, BN, TN> FB;
     // One k tile: the next one is on its way into wr while rd is read.  (wr and rd never overlap, and __restrict says so: otherwise every
-    // LDS read would wait for the loads.)
+    // LDS read would wait for the loads.)  Four phases; each reads the fragments of the following one between its matrix instructions.  The
+    // first still multiplies the previous tile's last fragments, so that the matrix units have work right behind the barrier.
+    struct Regs { typename FA::type a[2][TM]; typename FB::type b[2][TN]; };
+    static __device__ __forceinline__ void phase(const LIN_LDS char* __restrict rd, const FA& fa, const FB& fb, Regs& r, f32x16 (&acc)[TM][TN], const int s) {
+        const int to = s & 1, from = to ^ 1;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) r.b[to][j] = fb.get(rd + SA, j, s);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) r.a[to][i] = fa.get(rd, i, s);
+        multiply(r, acc, from);
+    }
+    static __device__ __forceinline__ void multiply(const Regs& r, f32x16 (&acc)[TM][TN], const int from) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = mfma<T>(r.b[from][j], r.a[from][i], acc[i][j]);
+    }
     static __device__ __forceinline__ void step(LIN_LDS char* __restrict wr, const LIN_LDS char* __restrict rd, TA& ta, TB& tb, const FA& fa,
-                                                const FB& fb, f32x16 (&acc)[TM][TN], bool more, int k_left, int wave) {
+                                                const FB& fb, Regs& r, f32x16 (&acc)[TM][TN], bool more, int k_left, int wave) {
         if (more) {
             ta.load(wr, k_left, wave);
             tb.load(wr + SA, k_left, wave);
         }
-        typename FA::type a[2][TM];
-        typename FB::type b[2][TN];
-#pragma unroll
-        for (int j = 0; j < TN; ++j) b[0][j] = fb.get(rd + SA, j, 0);
-#pragma unroll
-        for (int i = 0; i < TM; ++i) a[0][i] = fa.get(rd, i, 0);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            if (s < 3) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j) b[(s + 1) & 1][j] = fb.get(rd + SA, j, s + 1);
-#pragma unroll
-                for (int i = 0; i < TM; ++i) a[(s + 1) & 1][i] = fa.get(rd, i, s + 1);
-            }
-#pragma unroll
-            for (int i = 0; i < TM; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = mfma<T>(b[s & 1][j], a[s & 1][i], acc[i][j]);
-            if (sizeof(T) == 2 && s < 3) {
-                // the next fragments are read between the matrix instructions and not in a row in front of them (1096 -> 1200 TFLOP/s at
-                // 8192 x 8192 x 4096, bf16)
-                constexpr int READS = (LA == KC ? TM : 2 * TM) + (LB == KC ? TN : 2 * TN), PER = (READS + TM * TN - 1) / (TM * TN);
+            phase(rd, fa, fb, r, acc, s);
+            if (sizeof(T) == 2) {
+                // reads and matrix instructions in turn, and not the reads in a row in front (1096 -> 1255 TFLOP/s at 8192 x 8192 x 4096, bf16,
+                // with the phases' overlap across the barrier)
 #pragma unroll
                 for (int q = 0; q < TM * TN; ++q) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);   // LDS reads
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);     // one matrix instruction
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one matrix instruction
                 }
             }
         }
     }
+    static __device__ __forceinline__ void fill(LIN_LDS char* __restrict l, const GemmP& p, const Item& it, TA& ta, TB& tb, int wave, int lane) {
+        ta.init(p.a, p.lda, it.tm * BM, p.M, p.K, it.kt0, wave, lane);
+        tb.init(p.b, p.ldb, it.tn * BN, p.N, p.K, it.kt0, wave, lane);
+        ta.load(l, p.K - it.kt0 * BK, wave);
+        tb.load(l + SA, p.K - it.kt0 * BK, wave);
+    }
+    // The epilogue of an item, with the next one's first tile on its way into `l`.  A wave turns its sums, 32 rows at a time, from a lane per row
+    // to rows in a row through its part of `turn` (32 rows of TN x 32 floats, 16-byte chunk c of row r at c ^ r): what follows then moves whole
+    // lines of C, and in a loop: unrolled over the sums' registers, the code alone cost some 10 us per launch and 4 us per tile.
+    static __device__ __forceinline__ void finish(LIN_LDS char* __restrict l, LIN_LDS char* __restrict turn, const GemmP& p, const Item& it, bool more,
+                                                  const Item& next, TA& ta, TB& tb, const f32x16 (&acc)[TM][TN], int wave, int lane) {
+        if (more) fill(l, p, next, ta, tb, wave, lane);
+        constexpr int CH = TN * 8, LPR = TN * 4, RPP = 64 / LPR, PASSES = 32 / RPP;   // chunks and lanes per row, rows per pass
+        typedef typename Mem8<T>::t M8;
+        LIN_LDS char* t = turn + wave * (32 * CH * 16);
+        const int n = it.tn * BN + (wave % WN) * (BN / WN) + (lane % LPR) * 8;
+        const bool whole = n + 8 <= p.N;
+        const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        const f32x8 bias = p.bias && whole && p.splits == 1 ? load8<T>(p.bias, n) : zero;
+        float* part = p.part + (int64_t)it.split * p.M * p.ld_part;   // (ld_part: whole groups of 8)
+#pragma unroll 1
+        for (int i = 0; i < TM; ++i) {
+            const int m0 = it.tm * BM + (wave / WN) * (BM / WM) + i * 32 + lane / LPR;
+            M8 res[PASSES];   // all of the block's residual is asked for before the first of it is needed
+            if (p.res && p.splits == 1 && whole) {
+#pragma unroll
+                for (int q = 0; q < PASSES; ++q) res[q] = *(const M8*)((const T*)p.res + min(m0 + q * RPP, p.M - 1) * p.ld_res + n);
+            }
+            const int r = lane & 31;
+#pragma unroll
+            for (int k = 0; k < TM; ++k) {   // (a loop over registers is one over branches)
+                if (k != i) continue;
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f32x4 v = {acc[k][j][4 * g], acc[k][j][4 * g + 1], acc[k][j][4 * g + 2], acc[k][j][4 * g + 3]};
+                        *(LIN_LDS f32x4*)(t + (r * CH + ((j * 8 + 2 * g + (lane >> 5)) ^ (r & (CH - 1)))) * 16) = v;
+                    }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < PASSES; ++q) {
+                const int row = q * RPP + lane / LPR, m = m0 + q * RPP, c = (lane % LPR) * 2;
+                const f32x4 lo = *(const LIN_LDS f32x4*)(t + (row * CH + (c ^ (row & (CH - 1)))) * 16);
+                const f32x4 hi = *(const LIN_LDS f32x4*)(t + (row * CH + ((c + 1) ^ (row & (CH - 1)))) * 16);
+                const f32x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                if (m < p.M) {
+                    if (p.splits > 1) {
+                        if (n < p.ld_part) *(f32x8*)(part + m * p.ld_part + n) = v;
+                    } else if (whole) {
+                        epilogue8<T>(p, m, n, v, bias, p.res ? __builtin_convertvector(res[q], f32x8) : zero);
+                    } else if (n < p.N) {
+                        epilogue1<T>(p, m, n, v);
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
 };
 
-// A work item is a tile of C and a part of k.  Workgroup w runs on XCD w % 8 (each has an L2 of its own), so every XCD gets a contiguous run
-// of items, walked in groups of 8 tile rows: the operands of the tiles in flight on one XCD stay in its L2.
+// Workgroup w runs on XCD w % 8 (each has an L2 of its own), so every XCD gets a contiguous run of items, walked in groups of 8 tile rows: the
+// operands of the tiles in flight on one XCD stay in its L2.
 template <class T, int LA, int LB, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_gemm(const GemmP p) {
     typedef Gemm<T, LA, LB, BM, BN, WM, WN> G;
@@ -296,35 +365,31 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_gemm(const GemmP p) 
     __shared__ __attribute__((aligned(1024))) char lds[2 * (SA + SB)];
     LIN_LDS char* L = (LIN_LDS char*)(LIN_LDS void*)lds;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave / WN, wn = wave % WN;
     const int gm = (p.M + BM - 1) / BM, gn = (p.N + BN - 1) / BN, tiles = gm * gn, items = tiles * p.splits;
     const int nk = (p.K + BK - 1) / BK, per_split = (nk + p.splits - 1) / p.splits;
     const int xcd = blockIdx.x & 7, per = items / 8, rest = items % 8;
     const int mine = per + (xcd < rest), base = xcd * per + min(xcd, rest), stride = (gridDim.x - xcd + 7) >> 3;
-    typename G::FA fa;
-    typename G::FB fb;
-    fa.init(wm * (BM / WM), lane);
-    fb.init(wn * (BN / WN), lane);
-    typename G::TA ta;
-    typename G::TB tb;
-    int tm = 0, tn = 0, kt0 = 0, kt1 = 0, split = 0;
-    auto begin = [&](int q) {   // the loads' side of item q of this XCD
-        const int id = base + q, t = id % tiles;
-        split = id / tiles;
+    auto locate = [&](int q) {   // item q of this XCD
         constexpr int GM = 8;
-        const int first = t / (GM * gn) * GM, gs = min(GM, gm - first), in = t - first * gn;
-        tm = first + in % gs;
-        tn = in / gs;
-        kt0 = split * per_split;
-        kt1 = min(nk, kt0 + per_split);
-        ta.init(p.a, p.lda, tm * BM, p.M, p.K, kt0, wave, lane);
-        tb.init(p.b, p.ldb, tn * BN, p.N, p.K, kt0, wave, lane);
-        ta.load(L, p.K - kt0 * BK, wave);
-        tb.load(L + SA, p.K - kt0 * BK, wave);
+        const int id = base + q, t = id % tiles, first = t / (GM * gn) * GM, gs = min(GM, gm - first), in = t - first * gn;
+        Item it;
+        it.tm = first + in % gs;
+        it.tn = in / gs;
+        it.split = id / tiles;
+        it.kt0 = it.split * per_split;
+        it.kt1 = min(nk, it.kt0 + per_split);
+        return it;
     };
     int q = blockIdx.x >> 3;
     if (q >= mine) return;   // (the same for the workgroup)
-    begin(q);
+    typename G::FA fa;
+    typename G::FB fb;
+    fa.init(wave / WN * (BM / WM), lane);
+    fb.init(wave % WN * (BN / WN), lane);
+    typename G::TA ta;
+    typename G::TB tb;
+    Item it = locate(q);
+    G::fill(L, p, it, ta, tb, wave, lane);
     while (true) {
         f32x16 acc[TM][TN];
 #pragma unroll
@@ -333,49 +398,55 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_gemm(const GemmP p) 
             for (int j = 0; j < TN; ++j)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+        typename G::Regs regs;   // (set 1 is multiplied before it is read for the first time: zeros)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) regs.a[1][i] = typename G::FA::type{};
+#pragma unroll
+        for (int j = 0; j < TN; ++j) regs.b[1][j] = typename G::FB::type{};
         uint32_t cur = 0;
-        for (int kt = kt0; kt < kt1; ++kt) {
-            __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this tile has arrived
-            __syncthreads();                      // ... for every wave, and all are done with the other one
-            G::step(L + (cur ^ (SA + SB)), L + cur, ta, tb, fa, fb, acc, kt + 1 < kt1, p.K - (kt + 1) * BK, wave);
-            cur ^= SA + SB;
-        }
+        __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the first tile has arrived
         __syncthreads();
-        const int m0 = tm * BM + wm * (BM / WM) + (lane & 31), n0 = tn * BN + wn * (BN / WN) + (lane >> 5) * 4, sp = split;
-        const bool more = q + stride < mine;
-        q += stride;
-        if (more) begin(q);   // the next item's first tile is on its way during the epilogue
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int m = m0 + i * 32;
-            if (m < p.M) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int n = n0 + j * 32 + e * 8;
-                        const f32x4 v = {acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
-                        if (n >= p.N) continue;
-                        if (p.splits > 1) *(f32x4*)(p.part + ((int64_t)sp * p.M + m) * p.ld_part + n) = v;   // (ld_part: a multiple of 4)
-                        else epilogue<T>(p, m, n, v);
-                    }
-            }
+        for (int kt = it.kt0; kt < it.kt1; ++kt) {
+            G::step(L + (cur ^ (SA + SB)), L + cur, ta, tb, fa, fb, regs, acc, kt + 1 < it.kt1, p.K - (kt + 1) * BK, wave);
+            cur ^= SA + SB;
+            __builtin_amdgcn_s_waitcnt(0x0F70);   // the next tile has arrived, for every wave, and all are done with this one
+            __syncthreads();
         }
+        G::multiply(regs, acc, 1);
+        q += stride;
+        const bool more = q < mine;
+        const Item next = more ? locate(q) : it;
+        G::finish(L, L + SA + SB, p, it, more, next, ta, tb, acc, wave, lane);
         if (!more) return;
+        it = next;
     }
 }
-// Sums the parts of k in their order, four columns a lane.
-template <class T>
+// Sums the parts of k: eight columns of a row per lane, S lanes over the parts (each its own in their order, then the S sums in theirs).
+template <class T, int S>
 __global__ void __launch_bounds__(256) k_linear_join(const GemmP p) {
-    const int cols = (p.N + 3) / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)p.M * cols) return;
-    const int m = (int)(i / cols), n = (int)(i % cols) * 4;
+    constexpr int C = 256 / S;
+    const int cols = (int)(p.ld_part / 8), part = threadIdx.x / C;
+    const int64_t i = (int64_t)blockIdx.x * C + threadIdx.x % C;
+    const bool in = i < (int64_t)p.M * cols;
+    const int m = in ? (int)(i / cols) : 0, n = in ? (int)(i % cols) * 8 : 0;
     const float* q = p.part + (int64_t)m * p.ld_part + n;
     const int64_t per = (int64_t)p.M * p.ld_part;
-    f32x4 s = *(const f32x4*)q;
-    for (int k = 1; k < p.splits; ++k) s += *(const f32x4*)(q + k * per);
-    epilogue<T>(p, m, n, s);
+    f32x8 s = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (in) {
+#pragma unroll 4
+        for (int k = part; k < p.splits; k += S) s += *(const f32x8*)(q + k * per);
+    }
+    if (S > 1) {
+        __shared__ float w[S][C][9];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[part][threadIdx.x % C][e] = s[e];
+        __syncthreads();
+        if (part) return;
+        for (int k = 1; k < S; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] += w[k][threadIdx.x][e];
+    }
+    if (in) epilogue<T>(p, m, n, s);
 }
 
 template <class T, int LA, int LB, int BM, int BN, int WM, int WN>
@@ -394,18 +465,23 @@ int launch_gemm_f32(const GemmP& p, int la, int lb, int tile, hipStream_t s);
 
 template <class T, int LA, int LB>
 int launch_gemm_l(const GemmP& p, int tile, hipStream_t s) {
-    constexpr int MANY = 0x7FFFFFFF;
     int rc = INSMOS_EINVAL;
     if constexpr (sizeof(T) == 2) {
         if (tile == T256) rc = launch_tile<T, LA, LB, 256, 256, 2, 4>(p, 256, s);   // one workgroup per CU, walking its items
     }
-    if (tile == T128) rc = launch_tile<T, LA, LB, 128, 128, 2, 2>(p, MANY, s);
-    if (tile == TNARROW) rc = launch_tile<T, LA, LB, 128, 32, 4, 1>(p, MANY, s);
-    if (tile == TFLAT) rc = launch_tile<T, LA, LB, 32, 128, 1, 4>(p, MANY, s);
+    if (tile == T128) rc = launch_tile<T, LA, LB, 128, 128, 2, 2>(p, 512, s);   // two per CU
+    if (tile == TNARROW) rc = launch_tile<T, LA, LB, 128, 32, 4, 1>(p, 1024, s);   // four
+    if (tile == TFLAT) rc = launch_tile<T, LA, LB, 32, 128, 1, 4>(p, 1024, s);
     if (rc != INSMOS_OK || p.splits == 1) return rc;
-    const int64_t threads = (int64_t)p.M * ((p.N + 3) / 4);
-    const auto kernel = k_linear_join<T>;
-    INSMOS_LAUNCH(kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, s, p);
+    const int64_t rows8 = (int64_t)p.M * (p.ld_part / 8);
+    // many parts are few results: 16 lanes each (469 parts of 64 x 128 fp32: 129 -> 9 us)
+    if (p.splits >= 16) {
+        const auto kernel = k_linear_join<T, 16>;
+        INSMOS_LAUNCH(kernel, dim3((unsigned)((rows8 + 15) / 16)), dim3(256), 0, s, p);
+    } else {
+        const auto kernel = k_linear_join<T, 1>;
+        INSMOS_LAUNCH(kernel, dim3((unsigned)((rows8 + 255) / 256)), dim3(256), 0, s, p);
+    }
     HIP_TRY(hipGetLastError());
     return INSMOS_OK;
 }

@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(256) k_linear_pack(const T* __restrict__ src, 
     typedef T TV __attribute__((ext_vector_type(16 / sizeof(T))));
     TV v;
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = c + e < cols ? src[r * ld + c + e] : (T)0.f;
+    for (int e = 0; e < V; ++e) v[e] = c + e < cols ? src[r * ld + c + e] : (T)0;
     *(TV*)(dst + r * ld_dst + c) = v;
 }
 struct Operand {
@@ -89,20 +89,17 @@ Plan plan_for(int M, int N, int K, int dtype) {
     }
     return r;
 }
-size_t plan_bytes(const Plan& r, int M, int N) { return r.splits > 1 ? pad256((size_t)r.splits * M * round_up(N, 4) * sizeof(float)) : 0; }
+size_t plan_bytes(const Plan& r, int M, int N) { return r.splits > 1 ? pad256((size_t)r.splits * M * round_up(N, 8) * sizeof(float)) : 0; }
 int run_gemm(GemmP p, const Operand& a, const Operand& b, int dtype, Bump& ws, hipStream_t s) {
     const Plan r = plan_for(p.M, p.N, p.K, dtype);
     p.a = a.p; p.lda = a.ld;
     p.b = b.p; p.ldb = b.ld;
     p.splits = r.splits;
     if (r.splits > 1) {
-        p.ld_part = round_up(p.N, 4);
+        p.ld_part = round_up(p.N, 8);
         p.part = ws.take<float>((size_t)r.splits * p.M * p.ld_part);
         if (!p.part) return INSMOS_EWORKSPACE;
     }
-    const uintptr_t es = size_of(dtype), four = 4 * es;
-    auto fits = [&](const void* q, int64_t ld) { return !q || ((uintptr_t)q % four == 0 && ld % 4 == 0); };
-    p.vec = fits(p.y, p.ld_y) && fits(p.z, p.ld_z) && fits(p.res, p.ld_res) && fits(p.bias, 0);
     return dtype == INSMOS_BF16 ? launch_gemm_bf16(p, a.lay, b.lay, r.tile, s)
            : dtype == INSMOS_F16 ? launch_gemm_f16(p, a.lay, b.lay, r.tile, s) : launch_gemm_f32(p, a.lay, b.lay, r.tile, s);
 }
@@ -117,46 +114,60 @@ struct SlopeP {
     int64_t M;
     int N, ld_part, act, rows;   // rows per workgroup
     int lanes;           // column lanes (a power of two <= 32)
-    int vec;
 };
 // 256 lanes = `lanes` over the columns (16 bytes each) x the rest over rows; dz rounds dy act'(z) once to the type (the products read it in that
 // type); the column sums are taken before the rounding, in fp32, rows in a fixed order.
 template <class T>
 __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {
     constexpr int V = 16 / sizeof(T);
-    typedef T TV __attribute__((ext_vector_type(16 / sizeof(T))));
+    typedef T TV __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));   // (16 bytes at any address)
     const int lanes = p.lanes, rl = 256 / lanes, cl = threadIdx.x % lanes, r0 = threadIdx.x / lanes;
     const int n = (blockIdx.x * lanes + cl) * V;
     const int64_t from = (int64_t)blockIdx.y * p.rows, to = min(p.M, from + p.rows);
     float sum[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
-    if (n < p.N) {
+    auto row = [&](int64_t m, const float (&d0)[V], const float (&zz)[V]) {
+        TV out;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            float d = d0[e];
+            if (p.act && n + e < p.N) d *= slope(zz[e], p.act);
+            sum[e] += d;
+            out[e] = (T)d;
+        }
+        if (p.dz) *(TV*)((T*)p.dz + m * p.ld_dz + n) = out;   // (dz rows are padded to whole chunks, with zeros)
+    };
+    if (n + V <= p.N) {
+        constexpr int U = 4;   // rows in flight
+        for (int64_t m = from + r0; m < to; m += U * rl) {
+            TV a[U], b[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t q = min(m + u * rl, to - 1);
+                a[u] = *(const TV*)((const T*)p.dy + q * p.ld_dy + n);
+                b[u] = p.z ? *(const TV*)((const T*)p.z + q * p.ld_z + n) : a[u];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (m + u * rl >= to) break;
+                float d[V], zz[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) { d[e] = (float)a[u][e]; zz[e] = (float)b[u][e]; }
+                row(m + u * rl, d, zz);
+            }
+        }
+    } else if (n < p.N) {
         for (int64_t m = from + r0; m < to; m += rl) {
             const T* dy = (const T*)p.dy + m * p.ld_dy + n;
             const T* z = p.z ? (const T*)p.z + m * p.ld_z + n : nullptr;
             float d[V], zz[V];
-            if (p.vec && n + V <= p.N) {
-                const TV a = *(const TV*)dy;
-                TV b = a;
-                if (z) b = *(const TV*)z;
-#pragma unroll
-                for (int e = 0; e < V; ++e) { d[e] = (float)a[e]; zz[e] = (float)b[e]; }
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    d[e] = n + e < p.N ? (float)dy[e] : 0.f;
-                    zz[e] = z && n + e < p.N ? (float)z[e] : 0.f;
-                }
-            }
-            TV out;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                if (p.act && n + e < p.N) d[e] *= slope(zz[e], p.act);
-                sum[e] += d[e];
-                out[e] = (T)d[e];
+                d[e] = n + e < p.N ? (float)dy[e] : 0.f;
+                zz[e] = z && n + e < p.N ? (float)z[e] : 0.f;
             }
-            if (p.dz) *(TV*)((T*)p.dz + m * p.ld_dz + n) = out;   // (dz rows are padded to whole chunks, with zeros)
+            row(m, d, zz);
         }
     }
     if (!p.part) return;
@@ -317,7 +328,6 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
             q.part = bump.take<float>((size_t)r.blocks * N);
             if (!q.part) return INSMOS_EWORKSPACE;
         }
-        q.vec = (uintptr_t)dy % 16 == 0 && ld_dy % chunk == 0 && (!q.z || ((uintptr_t)z % 16 == 0 && ld_z % chunk == 0));
         rc = dtype == INSMOS_F32 ? run_slope_t<float>(q, r, db, s)
              : dtype == INSMOS_BF16 ? run_slope_t<__bf16>(q, r, db, s) : run_slope_t<_Float16>(q, r, db, s);
         if (rc != INSMOS_OK) return rc;
