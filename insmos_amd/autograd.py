@@ -487,51 +487,20 @@ def mos_loss(logits, gt_labels, n_classes=3, ignore_index=(0,)):
 # ---------------------------------------------------------------------------------------------------------------------
 # pointwise layer: product + bias + activation + residual in one kernel (csrc/linear.hip)
 # ---------------------------------------------------------------------------------------------------------------------
-_LINEAR_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_host_module = None
 
 
-def _rows(t, cols, shared=False):
-    """t as (rows, cols) whose rows are contiguous and do not overlap (shared: they may be one row), and the row pitch in elements.  A copy
-    only where t is not so."""
-    t = t.reshape(-1, cols)
-    if (t.shape[1] != 1 and t.stride(1) != 1) or (t.shape[0] != 1 and not (cols <= t.stride(0) <= 1 << 20 or (shared and t.stride(0) == 0))):
-        t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] != 1 else cols)
-
-
-def _weight_layout(w):
-    """(weight, its row pitch, 1 if it lies as (cout, cin) in memory)"""
-    cin, cout = w.shape
-    if w.stride(1) == 1 and cout <= w.stride(0) <= 1 << 20:
-        return w, w.stride(0), 0
-    if w.stride(0) == 1 and cin <= w.stride(1) <= 1 << 20:
-        return w, w.stride(1), 1
-    return w.contiguous(), cout, 0
-
-
-def _linear_forward(x, weight, bias, residual, act, residual_first, keep_z):
-    """(y, z or None) of checked arguments."""
-    lib = _lib.load()
-    cin, cout = weight.shape
-    x2, ld_x = _rows(x, cin)
-    n = x2.shape[0]
-    dt = _LINEAR_DTYPES[x.dtype]
-    y = torch.empty(x.shape[:-1] + (cout,), dtype=x.dtype, device=x.device)
-    z = torch.empty((n, cout), dtype=x.dtype, device=x.device) if keep_z else None
-    if n == 0 or cout == 0:
-        return y, z
-    w2, ld_w, out_in = _weight_layout(weight)
-    r2, ld_r = _rows(residual, cout, shared=True) if residual is not None else (None, 0)
-    b = bias.contiguous() if bias is not None else None
-    with torch.cuda.device(x.device):
-        need = lib.insmos_linear_ws_bytes(n, cin, cout, dt)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-        _lib.check(lib.insmos_linear(x2.data_ptr(), ld_x, w2.data_ptr(), ld_w, out_in, b.data_ptr() if b is not None else None,
-                                     r2.data_ptr() if r2 is not None else None, ld_r, 1 if residual_first else 0, act, n, cin, cout, dt,
-                                     y.data_ptr(), cout, z.data_ptr() if z is not None else None, cout, ws.data_ptr(), need,
-                                     _stream(x.device)), "insmos_linear")
-    return y, z
+def _host():
+    """The C++ side of linear(): argument checks, allocations and the library call (csrc/host_tensors.cpp)."""
+    global _host_module
+    if _host_module is None:
+        lib = _lib.load()
+        from . import _host as m
+        m.bind_linear(*[ctypes.cast(f, ctypes.c_void_p).value for f in (lib.insmos_linear, lib.insmos_linear_ws_bytes,
+                                                                        lib.insmos_linear_backward, lib.insmos_linear_backward_ws_bytes)])
+        _host_module = m
+    return _host_module
 
 
 class LinearFunction(torch.autograd.Function):
@@ -542,9 +511,9 @@ class LinearFunction(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act, residual_first):
         # relu: y > 0 says what z > 0 does, unless a residual was added behind it
         of_y = act == 1 and (residual is None or residual_first)
-        y, z = _linear_forward(x, weight, bias, residual, act, residual_first, act != 0 and not of_y)
+        y, z = _host().linear_forward(x, weight, bias, residual, act, residual_first, act != 0 and not of_y)
         ctx.save_for_backward(x, weight, y if of_y else z)
-        ctx.meta = (act, bool(residual_first), bias is not None, residual is not None)
+        ctx.meta = (act, residual_first, bias is not None, residual is not None)
         return y
 
     @staticmethod
@@ -553,77 +522,27 @@ class LinearFunction(torch.autograd.Function):
         x, weight, z = ctx.saved_tensors
         act, first, has_bias, has_res = ctx.meta
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        cin, cout = weight.shape
-        x2, ld_x = _rows(x, cin)
-        n = x2.shape[0]
-        dev, dtype = x.device, x.dtype
-        dx = torch.empty((n, cin), dtype=dtype, device=dev) if need_x else None
-        db = torch.empty((cout,), dtype=dtype, device=dev) if need_b and has_bias else None
-        w2, ld_w, out_in = _weight_layout(weight)
-        dw = None
-        if need_w:
-            dw = torch.empty((cout, cin) if out_in else (cin, cout), dtype=dtype, device=dev)
-        own_dz = need_r and has_res and first and act != 0
-        chunk = 16 // x.element_size()
-        ld_z = -(-cout // chunk) * chunk
-        if n == 0 or cout == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-            dz = dy
-        else:
-            lib = _lib.load()
-            dt = _LINEAR_DTYPES[dtype]
-            d2, ld_d = _rows(dy, cout)
-            z2, ld_s = (z.reshape(-1, cout), cout) if z is not None else (None, 0)
-            with torch.cuda.device(dev):
-                dz = torch.empty((n, ld_z), dtype=dtype, device=dev) if own_dz else None
-                if dx is not None or dw is not None or db is not None or own_dz:
-                    need = lib.insmos_linear_backward_ws_bytes(n, cin, cout, dt)
-                    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-                    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-                    _lib.check(lib.insmos_linear_backward(d2.data_ptr(), ld_d, ptr(z2), ld_s, x2.data_ptr(), ld_x, w2.data_ptr(), ld_w, out_in,
-                                                          act, n, cin, cout, dt, ptr(dx), cin, ptr(dw), cin if out_in else cout, ptr(db),
-                                                          ptr(dz), ld_z, ws.data_ptr(), need, _stream(dev)), "insmos_linear_backward")
-        dr = None
-        if need_r and has_res:
-            dr = dz[:, :cout].reshape(dy.shape) if own_dz and n and cout else dy
-        return (dx.reshape(x.shape) if dx is not None else None, dw.t() if dw is not None and out_in else dw, db, dr, None, None)
+        need_r = need_r and has_res
+        dx, dw, db, dz = _host().linear_backward(dy, z, x, weight, act, need_x, need_w, need_b and has_bias, need_r and first and act != 0)
+        return dx, dw, db, (dz if dz is not None else dy) if need_r else None, None, None
 
 
 def linear(x, weight, bias=None, residual=None, activation=None, residual_first=False):
-    """Pointwise layer y = act(x @ weight + bias) + residual, or act(x @ weight + bias + residual) with residual_first, in one product kernel
-    (forward) and three launches of it and its surroundings (backward).
+    """Pointwise layer y = act(x @ weight + bias) + residual, or act(x @ weight + bias + residual) with residual_first: one launch (two where
+    few tiles share a long cin) forward, and backward dz with the bias gradient, then a product each for x and weight.
 
     x (..., cin): rows of any pitch; weight (cin, cout), one tap of sparse_conv(); an nn.Linear weight's transpose (a (cout, cin) tensor's
     .t()) is read as it lies.  bias (cout,).  residual: the output's shape (an expanded one works: rows of pitch 0).  activation: None,
     "relu", "gelu" (erf), "gelu_tanh" or "silu".  All tensors of one dtype -- float32, bfloat16 or float16 -- on one GPU; sums in fp32.
-    Widths up to 2^20.  Differentiable once in all four tensors; without gradients nothing is kept for a backward pass."""
-    if activation not in _ACTIVATIONS:
-        raise ValueError(f"linear: activation is one of {[a for a in _ACTIVATIONS]}, not {activation!r}")
-    if x.dtype not in _LINEAR_DTYPES:
-        raise ValueError(f"linear: float32, bfloat16 or float16, not {x.dtype}")
-    if x.device.type != "cuda":
-        raise ValueError(f"linear: tensors on the GPU, not on {x.device}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
-        raise ValueError(f"linear: x (..., cin) and weight (cin, cout), not {tuple(x.shape)} and {tuple(weight.shape)}")
-    cin, cout = weight.shape
-    if cin < 1 or cin > 1 << 20 or cout > 1 << 20:
-        raise ValueError(f"linear: widths from 1 to 2^20, not {cin} -> {cout}")
-    if x.numel() // cin > 0x7FFFFF00:
-        raise ValueError(f"linear: at most {0x7FFFFF00} rows")
-    if bias is not None and tuple(bias.shape) != (cout,):
-        raise ValueError(f"linear: bias ({cout},), not {tuple(bias.shape)}")
-    if residual is not None and residual.shape != x.shape[:-1] + (cout,):
-        raise ValueError(f"linear: residual {tuple(x.shape[:-1]) + (cout,)}, not {tuple(residual.shape)}")
-    for name, t in (("weight", weight), ("bias", bias), ("residual", residual)):
-        if t is not None and (t.dtype != x.dtype or t.device != x.device):
-            raise ValueError(f"linear: {name} is {t.dtype} on {t.device}, x {x.dtype} on {x.device}")
-    act = _ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
-                                    (residual is not None and residual.requires_grad)):
+    Widths up to 2^20.  Differentiable once in all four tensors; without gradients nothing is kept for a backward pass.  In 16 bits the
+    backward rounds z (for the slope) and dz (for the products) once each."""
+    try:
+        act = _ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"linear: activation is one of {list(_ACTIVATIONS)}, not {activation!r}") from None
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         return LinearFunction.apply(x, weight, bias, residual, act, bool(residual_first))
-    return _linear_forward(x, weight, bias, residual, act, bool(residual_first), False)[0]
+    return _host().linear_forward(x, weight, bias, residual, act, residual_first, False)[0]
 
 
 # ---------------------------------------------------------------------------------------------------------------------

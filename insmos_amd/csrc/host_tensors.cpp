@@ -1,12 +1,18 @@
-// insmos_amd/csrc/host_tensors.cpp -- the host side of the optimiser step that touches every tensor: one pass in C++ over Python lists of
-// tensors that checks them and writes the InsmosOptTensor table (include/insmos_hip.h).  From Python the same pass costs ten attribute
-// reads per tensor (some 0.1 us each: 0.5 ms for 250 tensors, ten times what the GPU needs for them).  Built as the extension module
+// insmos_amd/csrc/host_tensors.cpp -- host sides that Python is too slow for, over torch's tensors.  Built as the extension module
 // insmos_amd._host; nothing here runs on the GPU.
+//   opt_table: one pass over the optimiser step's lists that checks them and writes the InsmosOptTensor table (include/insmos_hip.h).  From
+//     Python the same pass costs ten attribute reads per tensor (some 0.1 us each: 0.5 ms for 250 tensors, ten times what the GPU needs).
+//   linear_forward / linear_backward: checks, allocations and the call of insmos_linear(_backward) (20 us from Python, where the GPU needs 7
+//     for one row).
 #include <Python.h>
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <exception>
+#include <stdexcept>
 #include <string>
 #include <utility>
 #include <vector>
@@ -125,7 +131,192 @@ PyObject* opt_table(PyObject*, PyObject* args) {
     return result;
 }
 
-PyMethodDef kMethods[] = {{"opt_table", opt_table, METH_VARARGS, "checks lists of tensors and writes their InsmosOptTensor table"}, {nullptr, nullptr, 0, nullptr}};
+// ---- linear -----------------------------------------------------------------------------------------------------------------
+decltype(&insmos_linear) g_linear = nullptr;
+decltype(&insmos_linear_ws_bytes) g_linear_ws = nullptr;
+decltype(&insmos_linear_backward) g_backward = nullptr;
+decltype(&insmos_linear_backward_ws_bytes) g_backward_ws = nullptr;
+
+// bind_linear(addresses of insmos_linear, _ws_bytes, _backward, _backward_ws_bytes)
+PyObject* bind_linear(PyObject*, PyObject* args) {
+    unsigned long long f[4];
+    if (!PyArg_ParseTuple(args, "KKKK", &f[0], &f[1], &f[2], &f[3])) return nullptr;
+    g_linear = (decltype(g_linear))f[0];
+    g_linear_ws = (decltype(g_linear_ws))f[1];
+    g_backward = (decltype(g_backward))f[2];
+    g_backward_ws = (decltype(g_backward_ws))f[3];
+    Py_RETURN_NONE;
+}
+std::string shape(const at::Tensor& t) {
+    std::string r = "(";
+    for (int64_t d = 0; d < t.dim(); ++d) r += (d ? ", " : "") + std::to_string(t.size(d));
+    return r + ")";
+}
+[[noreturn]] void refuse(const std::string& t) { throw Refused("linear: " + t); }
+const at::Tensor& arg(PyObject* o, const char* name) {
+    if (!THPVariable_Check(o)) refuse(std::string(name) + " is no tensor");
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (t.layout() != c10::kStrided) refuse(std::string(name) + " is sparse");
+    return t;
+}
+constexpr int64_t kMost = 1 << 20;   // widths and pitches
+// t as rows of `cols` whose values are contiguous and that do not overlap (shared: they may be one row), and their pitch; a copy only where t
+// is not so
+struct Rows { at::Tensor t; int64_t n, ld; };
+Rows rows_of(const at::Tensor& t, int64_t cols, bool shared = false) {
+    at::Tensor v = t.dim() == 2 ? t : t.reshape({-1, cols});
+    const int64_t n = v.size(0);
+    if ((cols != 1 && v.stride(1) != 1) || (n != 1 && !((v.stride(0) >= cols && v.stride(0) <= kMost) || (shared && v.stride(0) == 0)))) v = v.contiguous();
+    return {v, n, n != 1 ? v.stride(0) : cols};
+}
+struct Weight { at::Tensor t; int64_t ld; int out_in; };
+Weight weight_of(const at::Tensor& w) {
+    const int64_t cin = w.size(0), cout = w.size(1);
+    if (w.stride(1) == 1 && w.stride(0) >= cout && w.stride(0) <= kMost) return {w, w.stride(0), 0};
+    if (w.stride(0) == 1 && w.stride(1) >= cin && w.stride(1) <= kMost) return {w, w.stride(1), 1};
+    return {w.contiguous(), cout, 0};
+}
+void* at_ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* stream_of(const at::Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+struct LibraryError : std::runtime_error { using std::runtime_error::runtime_error; };
+void checked(int rc, const char* what) {
+    if (rc != 0)
+        throw LibraryError(std::string(what) + " failed: " + (rc == INSMOS_EINVAL ? "INSMOS_EINVAL (bad argument)" : rc == INSMOS_EHIP ? "INSMOS_EHIP (HIP runtime error)"
+                                                              : rc == INSMOS_EWORKSPACE ? "INSMOS_EWORKSPACE" : std::to_string(rc)));
+}
+// an exception class by name
+void raise(const char* module, const char* name, const char* text) {
+    PyObject* m = PyImport_ImportModule(module);
+    PyObject* kind = m ? PyObject_GetAttrString(m, name) : nullptr;
+    if (kind) PyErr_SetString(kind, text);   // (else the import's own error stands)
+    Py_XDECREF(kind);
+    Py_XDECREF(m);
+}
+PyObject* wrap(const at::Tensor& t) {
+    if (t.defined()) return THPVariable_Wrap(t);
+    Py_RETURN_NONE;
+}
+template <class F>
+PyObject* guarded(F f) {   // no C++ exception leaves the module
+    try {
+        return f();
+    } catch (const Refused& e) {
+        PyErr_SetString(PyExc_ValueError, e.what());
+    } catch (const LibraryError& e) {
+        raise("insmos_amd._lib", "InsmosHipError", e.what());
+    } catch (const c10::OutOfMemoryError& e) {
+        raise("torch", "OutOfMemoryError", e.what_without_backtrace());   // as torch's own allocations do
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        PyErr_SetString(PyExc_RuntimeError, "linear failed");
+    }
+    return nullptr;
+}
+// rows of a buffer of the module's own start on 16 bytes
+int64_t padded(int64_t cols, const at::Tensor& like) {
+    const int64_t chunk = 16 / (int64_t)like.element_size();
+    return (cols + chunk - 1) / chunk * chunk;
+}
+
+// linear_forward(x, weight, bias or None, residual or None, act, residual_first, keep_z) -> (y, z or None)
+PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 7 || !g_linear) refuse("internal call");
+        const at::Tensor &x = arg(a[0], "x"), &w = arg(a[1], "weight");
+        const int act = (int)PyLong_AsLong(a[4]), first = PyObject_IsTrue(a[5]), keep = PyObject_IsTrue(a[6]);
+        const int dt = dtype_code(x.scalar_type());
+        std::string buf;
+        if (dt < 0) refuse(std::string("float32, bfloat16 or float16, not ") + place(x, buf));
+        if (!x.is_cuda()) refuse("tensors on the GPU, not on " + x.device().str());
+        if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(0)) refuse("x (..., cin) and weight (cin, cout), not " + shape(x) + " and " + shape(w));
+        const int64_t cin = w.size(0), cout = w.size(1);
+        if (cin < 1 || cin > kMost || cout > kMost) refuse("widths from 1 to 2^20, not " + std::to_string(cin) + " -> " + std::to_string(cout));
+        auto same = [&](const at::Tensor& t, const char* name) {
+            std::string b1, b2;
+            if (t.scalar_type() != x.scalar_type() || t.device() != x.device())
+                refuse(std::string(name) + " is " + place(t, b1) + ", x " + place(x, b2));
+        };
+        same(w, "weight");
+        std::vector<int64_t> out(x.sizes().begin(), x.sizes().end());
+        out.back() = cout;
+        at::Tensor b, r;
+        if (a[2] != Py_None) {
+            b = arg(a[2], "bias");
+            same(b, "bias");
+            if (b.dim() != 1 || b.size(0) != cout) refuse("bias (" + std::to_string(cout) + ",), not " + shape(b));
+            b = b.contiguous();
+        }
+        if (a[3] != Py_None) {
+            r = arg(a[3], "residual");
+            same(r, "residual");
+            if (r.sizes() != at::IntArrayRef(out)) refuse("residual of the output's shape, not " + shape(r));
+        }
+        if (x.numel() / cin > 0x7FFFFF00) refuse("at most " + std::to_string(0x7FFFFF00) + " rows");
+        c10::DeviceGuard guard(x.device());
+        at::Tensor y = at::empty(out, x.options().requires_grad(false)), z;
+        const int64_t n = x.numel() / cin, ld_z = padded(cout, x);
+        if (keep) z = at::empty({n, ld_z}, x.options().requires_grad(false));
+        if (n && cout) {
+            const Rows xr = rows_of(x, cin);
+            const Weight wt = weight_of(w);
+            Rows rr{};
+            if (r.defined()) rr = rows_of(r, cout, true);
+            const size_t need = g_linear_ws(n, (int)cin, (int)cout, dt);
+            const at::Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
+            checked(g_linear(xr.t.data_ptr(), xr.ld, wt.t.data_ptr(), wt.ld, wt.out_in, at_ptr(b), at_ptr(rr.t), rr.ld, first, act, n, (int)cin, (int)cout,
+                             dt, y.data_ptr(), cout, at_ptr(z), ld_z, at_ptr(ws), need, stream_of(x)), "insmos_linear");
+        }
+        return Py_BuildValue("NN", wrap(y), wrap(z));
+    });
+}
+// linear_backward(dy, z or None, x, weight, act, need_x, need_w, need_b, need_dz) -> (dx, dweight, dbias, dz), None where not needed
+PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 9 || !g_backward) refuse("internal call");
+        const at::Tensor &dy = arg(a[0], "the gradient"), &x = arg(a[2], "x"), &w = arg(a[3], "weight");
+        at::Tensor z;
+        if (a[1] != Py_None) z = arg(a[1], "z");
+        const int act = (int)PyLong_AsLong(a[4]);
+        const bool need_x = PyObject_IsTrue(a[5]), need_w = PyObject_IsTrue(a[6]), need_b = PyObject_IsTrue(a[7]), need_dz = PyObject_IsTrue(a[8]);
+        const int dt = dtype_code(x.scalar_type());
+        const int64_t cin = w.size(0), cout = w.size(1), n = x.numel() / cin, ld_z = padded(cout, x);
+        if (dy.scalar_type() != x.scalar_type() || dy.device() != x.device()) refuse("the gradient is of another type or device than the output");
+        c10::DeviceGuard guard(x.device());
+        const auto opt = x.options().requires_grad(false);
+        const Weight wt = weight_of(w);
+        at::Tensor dx, dw, db, dz;
+        if (need_x) dx = at::empty(x.sizes(), opt);
+        if (need_w) dw = wt.out_in ? at::empty({cout, cin}, opt) : at::empty({cin, cout}, opt);
+        if (need_b) db = at::empty({cout}, opt);
+        if (n && cout) {
+            if (need_dz) dz = at::empty({n, ld_z}, opt);
+            if (need_x || need_w || need_b || need_dz) {
+                const Rows d = rows_of(dy, cout), xr = rows_of(x, cin);
+                const size_t need = g_backward_ws(n, (int)cin, (int)cout, dt);
+                const at::Tensor ws = at::empty({(int64_t)need}, opt.dtype(at::kByte));
+                checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(z), z.defined() ? (z.dim() == 2 && z.size(1) == ld_z ? ld_z : cout) : 0, xr.t.data_ptr(), xr.ld,
+                                   wt.t.data_ptr(), wt.ld, wt.out_in, act, n, (int)cin, (int)cout, dt, at_ptr(dx), cin, at_ptr(dw),
+                                   wt.out_in ? cin : cout, at_ptr(db), at_ptr(dz), ld_z, ws.data_ptr(), need, stream_of(x)),
+                        "insmos_linear_backward");
+            }
+            if (need_dz) dz = dz.narrow(1, 0, cout).reshape(dy.sizes());
+        } else {
+            if (need_x) dx.zero_();
+            if (need_w) dw.zero_();
+            if (need_b) db.zero_();
+            if (need_dz) dz = at::empty(dy.sizes(), opt);
+        }
+        if (need_w && wt.out_in) dw = dw.t();
+        return Py_BuildValue("NNNN", wrap(dx), wrap(dw), wrap(db), wrap(dz));
+    });
+}
+
+PyMethodDef kMethods[] = {{"opt_table", opt_table, METH_VARARGS, "checks lists of tensors and writes their InsmosOptTensor table"},
+                          {"bind_linear", bind_linear, METH_VARARGS, "addresses of the library's functions"},
+                          {"linear_forward", (PyCFunction)(void (*)())linear_forward, METH_FASTCALL, "checks and insmos_linear"},
+                          {"linear_backward", (PyCFunction)(void (*)())linear_backward, METH_FASTCALL, "insmos_linear_backward"},
+                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 }  // namespace
 

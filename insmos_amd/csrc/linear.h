@@ -36,7 +36,7 @@ template <> struct Mem8<__bf16> { typedef __bf16 t __attribute__((ext_vector_typ
 template <> struct Mem8<_Float16> { typedef _Float16 t __attribute__((ext_vector_type(8), aligned(2))); };
 
 enum { KC = 0, NC = 1 };                                            // which index of an operand is contiguous
-enum { T256 = 0, T128 = 1, TNARROW = 2, TFLAT = 3 };                // tiles 256x256, 128x128, 128x32 (few columns), 32x128 (few rows)
+enum { T256 = 0, T128 = 1, TNARROW = 2, TFLAT = 3, FEW = 4 };       // tiles 256x256, 128x128, 128x32 (few columns), 32x128 (few rows); k_linear_few
 
 struct GemmP {
     const void* a;
@@ -61,18 +61,41 @@ struct GemmP {
 // (v_exp and v_rcp: 1 ulp each; exp(-x) = inf gives 0)
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 constexpr float kGelu0 = 0.7978845608028654f, kGelu1 = 0.044715f;   // sqrt(2 / pi) (z + 0.044715 z^3)
+// Phi(-|z|) of the normal distribution, and e = exp(-z^2 / 2): a polynomial in t = 1 / (1 + 0.3 |z|) times e, fitted to the least largest relative
+// error (1.5e-7 for |z| <= 14, where the value leaves fp32's range).  The tail keeps its relative precision, which 1 + erf(z / sqrt 2) loses, in
+// less than half of erff's instructions.
+__device__ __forceinline__ float normal_tail(float z, float& e) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3f, fabsf(z), 1.f));
+    float p = fmaf(0.0356761676f, t, -0.157209128f);
+    p = fmaf(p, t, 0.206364304f);
+    p = fmaf(p, t, -0.0536939024f);
+    p = fmaf(p, t, 0.128567206f);
+    p = fmaf(p, t, 0.0999117609f);
+    p = fmaf(p, t, 0.120754239f);
+    p = fmaf(p, t, 0.11962928f);
+    e = __expf(-0.5f * z * z);
+    return p * t * e;
+}
 // act != INSMOS_ACT_NONE.  z times a weight between 0 and 1; silu's and the tanh form's are sigmoids: (1 + tanh u) / 2 = sigmoid(2 u).  (One formula for both: the
 // epilogue's code is part of every tile's time when it has to be fetched.)
 __device__ __forceinline__ float activate(float z, int act) {
     if (act == INSMOS_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-    if (act == INSMOS_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.7071067811865476f));
+    if (act == INSMOS_ACT_GELU) {
+        float e;
+        const float tail = normal_tail(z, e);
+        return z * (z > 0.f ? 1.f - tail : tail);
+    }
     const float c0 = act == INSMOS_ACT_SILU ? 1.f : 2.f * kGelu0, c1 = act == INSMOS_ACT_SILU ? 0.f : 2.f * kGelu0 * kGelu1;
     return z * sigmoid(z * (c0 + c1 * (z * z)));
 }
 __device__ __forceinline__ float slope(float z, int act) {
     switch (act) {
         case INSMOS_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case INSMOS_ACT_GELU: return 0.5f * (1.f + erff(z * 0.7071067811865476f)) + z * __expf(-0.5f * z * z) * 0.3989422804014327f;
+        case INSMOS_ACT_GELU: {
+            float e;
+            const float tail = normal_tail(z, e);
+            return (z > 0.f ? 1.f - tail : tail) + z * e * 0.3989422804014327f;
+        }
         case INSMOS_ACT_GELU_TANH: {
             const float s = sigmoid(2.f * kGelu0 * (z + kGelu1 * z * z * z));
             return s + z * 2.f * s * (1.f - s) * kGelu0 * (1.f + 3.f * kGelu1 * z * z);
@@ -449,6 +472,160 @@ __global__ void __launch_bounds__(256) k_linear_join(const GemmP p) {
     if (in) epilogue<T>(p, m, n, s);
 }
 
+// ---- few rows ---------------------------------------------------------------------------------------------------------------
+// Up to 32 rows of x (tokens being generated): the weights' bytes are the time.  One launch, no workspace, any alignment: a workgroup has 32
+// columns and all of k, its 8 waves take 128 bytes of k in turn and add up in LDS.  Fragments come straight from memory (KC) or, for weights
+// with contiguous columns, through a turn of 16 x 32 values in the wave's own LDS; the whole of a wave's weights is in flight at once.
+// Rows and columns behind the matrix repeat the last one and are not stored; k behind its end is zero in both operands.
+// 1 x 2048 x 8192 bf16: %s against %s us with the flat tiles and a join.
+// eight values from k on, zeros behind K, one by one
+template <class T>
+__device__ __forceinline__ s16x8 load_k8(const T* row, int k, int K) {
+    s16x8 r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {   // (K > 0; no branch around the loads)
+        const short v = ((const short*)row)[min(k + e, K - 1)];
+        r[e] = k + e < K ? v : (short)0;
+    }
+    return r;
+}
+template <class T, int LB>
+struct Few {   // 16 bit: a chunk is 64 k, four steps of 16
+    static constexpr int CHUNK = 64, TURN = 4 * 1024;
+    typedef s16x8 type;
+    // (whole chunks without a branch: their loads all leave before the first is waited for)
+    static __device__ __forceinline__ void load_x(const T* row, int k0, int K, int lane, s16x8 (&f)[4]) {
+        typedef short M8 __attribute__((ext_vector_type(8), aligned(2)));
+        if (k0 + CHUNK <= K) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) f[s] = *(const M8*)((const short*)row + k0 + 16 * s + 8 * (lane >> 5));
+        } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) f[s] = load_k8(row, k0 + 16 * s + 8 * (lane >> 5), K);
+        }
+    }
+    static __device__ __forceinline__ void load_w(const T* w, int64_t ld, int n0, int N, int k0, int K, int lane, s16x8 (&f)[4]) {
+        if (LB == KC) {
+            load_x(w + (int64_t)min(n0 + (lane & 31), N - 1) * ld, k0, K, lane, f);
+        } else {
+            typedef short M8 __attribute__((ext_vector_type(8), aligned(2)));
+            const int n = n0 + (lane & 3) * 8;
+            if (k0 + CHUNK <= K && n0 + 32 <= N) {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) f[s] = *(const M8*)((const short*)w + (k0 + 16 * s + (lane >> 2)) * ld + n);
+            } else {
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int k = k0 + 16 * s + (lane >> 2);
+                    f[s] = k < K && n < N ? load_k8(w + k * ld, n, N) : s16x8{};
+                }
+            }
+        }
+    }
+    // the fragments of what load_w loaded
+    static __device__ __forceinline__ void turn(LIN_LDS char* l, int lane, s16x8 (&f)[4]) {
+        if (LB == KC) return;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) *(LIN_LDS s16x8*)(l + s * 1024 + lane * 16) = f[s];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int g = lane >> 4, j = lane & 15, k = (g >> 1) * 8 + (j >> 2), col = (g & 1) * 16 + 4 * (j & 3);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LIN_LDS s16x4*)(l + s * 1024 + k * 64 + col * 2));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LIN_LDS s16x4*)(l + s * 1024 + (k + 4) * 64 + col * 2));
+            f[s] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+};
+template <int LB>
+struct Few<float, LB> {   // fp32: a chunk is 32 k, four steps of 8 (their k in the order of Frag<float>)
+    static constexpr int CHUNK = 32, TURN = 0;
+    typedef f32x4 type;
+    static __device__ __forceinline__ void load_x(const float* row, int k0, int K, int lane, f32x4 (&f)[4]) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            constexpr int K4[4] = {0, 4, 1, 5};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = k0 + 8 * s + 2 * (lane >> 5) + K4[e];
+                const float v = row[min(k, K - 1)];
+                f[s][e] = k < K ? v : 0.f;
+            }
+        }
+    }
+    static __device__ __forceinline__ void load_w(const float* w, int64_t ld, int n0, int N, int k0, int K, int lane, f32x4 (&f)[4]) {
+        const int n = min(n0 + (lane & 31), N - 1);
+        if (LB == KC) return load_x(w + n * ld, k0, K, lane, f);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            constexpr int K4[4] = {0, 4, 1, 5};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = k0 + 8 * s + 2 * (lane >> 5) + K4[e];
+                const float v = w[min(k, K - 1) * ld + n];
+                f[s][e] = k < K ? v : 0.f;
+            }
+        }
+    }
+    static __device__ __forceinline__ void turn(LIN_LDS char*, int, f32x4 (&)[4]) {}
+};
+template <class T, int LB>
+__global__ void __launch_bounds__(512) k_linear_few(const GemmP p) {
+    typedef Few<T, LB> F;
+    constexpr int WAVES = 8;
+    __shared__ __attribute__((aligned(1024))) char lds[WAVES * (F::TURN > 4096 ? F::TURN : 4096)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // neighbouring columns on one XCD: they share lines
+    const int blocks = gridDim.x, xcd = blockIdx.x & 7, b = xcd * (blocks / 8) + min(xcd, blocks % 8) + (blockIdx.x >> 3), n0 = b * 32;
+    const T* x = (const T*)p.a + (int64_t)min(lane & 31, p.M - 1) * p.lda;
+    const T* w = (const T*)p.b;
+    LIN_LDS char* L = (LIN_LDS char*)(LIN_LDS void*)lds;
+    f32x16 acc;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+    const int chunks = (p.K + F::CHUNK - 1) / F::CHUNK;
+    typename F::type fx[2][4], fw[2][4];
+    if (wave < chunks) {
+        F::load_w(w, p.ldb, n0, p.N, wave * F::CHUNK, p.K, lane, fw[0]);
+        F::load_x(x, wave * F::CHUNK, p.K, lane, fx[0]);
+    }
+    for (int c = wave; c < chunks; c += 2 * WAVES) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int at = c + h * WAVES, next = at + WAVES;
+            if (at >= chunks) break;
+            if (next < chunks) {
+                F::load_w(w, p.ldb, n0, p.N, next * F::CHUNK, p.K, lane, fw[h ^ 1]);
+                F::load_x(x, next * F::CHUNK, p.K, lane, fx[h ^ 1]);
+            }
+            F::turn(L + wave * F::TURN, lane, fw[h]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) acc = mfma<T>(fw[h][s], fx[h][s], acc);
+        }
+    }
+    __syncthreads();
+    // sums of the waves: [wave][row 32][column 32], 16-byte chunk c of row r at c ^ (r & 7)
+    const int r = lane & 31;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const f32x4 v = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+        *(LIN_LDS f32x4*)(L + wave * 4096 + r * 128 + (((2 * g + (lane >> 5)) ^ (r & 7)) << 4)) = v;
+    }
+    __syncthreads();
+    const int m = threadIdx.x >> 2, c = (threadIdx.x & 3) * 2, n = n0 + c * 4;
+    if (m >= p.M || n >= p.N) return;   // (m < 32 of the 128)
+    f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
+#pragma unroll
+    for (int q = 0; q < WAVES; ++q) {
+        lo += *(const LIN_LDS f32x4*)(L + q * 4096 + m * 128 + ((c ^ (m & 7)) << 4));
+        hi += *(const LIN_LDS f32x4*)(L + q * 4096 + m * 128 + (((c + 1) ^ (m & 7)) << 4));
+    }
+    epilogue<T>(p, m, n, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 template <class T, int LA, int LB, int BM, int BN, int WM, int WN>
 int launch_tile(const GemmP& p, int most, hipStream_t s) {
     const int64_t items = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN) * p.splits;
@@ -466,6 +643,14 @@ int launch_gemm_f32(const GemmP& p, int la, int lb, int tile, hipStream_t s);
 template <class T, int LA, int LB>
 int launch_gemm_l(const GemmP& p, int tile, hipStream_t s) {
     int rc = INSMOS_EINVAL;
+    if constexpr (LA == KC) {
+        if (tile == FEW) {
+            const auto kernel = k_linear_few<T, LB>;
+            INSMOS_LAUNCH(kernel, dim3((unsigned)((p.N + 31) / 32)), dim3(512), 0, s, p);
+            HIP_TRY(hipGetLastError());
+            return INSMOS_OK;
+        }
+    }
     if constexpr (sizeof(T) == 2) {
         if (tile == T256) rc = launch_tile<T, LA, LB, 256, 256, 2, 4>(p, 256, s);   // one workgroup per CU, walking its items
     }

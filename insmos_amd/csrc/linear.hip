@@ -43,10 +43,10 @@ bool loadable(const void* p, int64_t ld, int contiguous, int lay, int dtype) {
 size_t packed_bytes(int64_t rows, int cols, int dtype) {
     return pad256((size_t)rows * round_up(cols, 16 / (int)size_of(dtype)) * size_of(dtype));
 }
-// `rows` x `cols` (cols contiguous) as a loadable operand; copies into ws where it is none
-int operand(const void* p, int64_t ld, int64_t rows, int cols, int lay, int dtype, Bump& ws, hipStream_t s, Operand* out) {
+// `rows` x `cols` (cols contiguous) as a loadable operand; copies into ws where it is none (any: the kernel takes it as it is)
+int operand(const void* p, int64_t ld, int64_t rows, int cols, int lay, int dtype, bool any, Bump& ws, hipStream_t s, Operand* out) {
     *out = {p, ld, lay};
-    if (loadable(p, ld, cols, lay, dtype)) return INSMOS_OK;
+    if (any || loadable(p, ld, cols, lay, dtype)) return INSMOS_OK;
     const int es = (int)size_of(dtype), to = round_up(cols, 16 / es);
     char* d = ws.take<char>((size_t)rows * to * es);
     if (!d) return INSMOS_EWORKSPACE;
@@ -65,11 +65,13 @@ struct Plan { int tile, splits; };
 // Rates of a full chip: 256x256 tiles 1200 TFLOP/s (bf16, one workgroup per CU), 128x128 1050 (two per CU); a launch takes as long as its fullest
 // CU, so the larger tile pays only where its tiles fill whole rounds of 256.  Up to 32 rows or columns the flat tiles waste least.
 // Where the tiles leave CUs idle, k is cut into parts, each at least 4 k tiles long, until about two workgroups per CU are there.
-Plan plan_for(int M, int N, int K, int dtype) {
+Plan plan_for(int M, int N, int K, int dtype, bool xw) {   // xw: the first operand has contiguous k
     const int bk = 128 / (int)size_of(dtype), nk = (K + bk - 1) / bk;
     Plan r = {T128, 1};
     int64_t tiles, want = 512;
     const int64_t t128 = (int64_t)((M + 127) / 128) * ((N + 127) / 128), t256 = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
+    // (one workgroup per 32 columns walks all of k: 16 x 8192 x 256 takes 25 us that way and 10 in parts)
+    if (M <= 32 && xw && (K <= 4096 || N >= 4096)) { r.tile = FEW; return r; }
     if (M <= 32) { r.tile = TFLAT; tiles = (N + 127) / 128; want = 1024; }
     else if (N <= 32) { r.tile = TNARROW; tiles = (M + 127) / 128; want = 1024; }
     else {
@@ -91,7 +93,7 @@ Plan plan_for(int M, int N, int K, int dtype) {
 }
 size_t plan_bytes(const Plan& r, int M, int N) { return r.splits > 1 ? pad256((size_t)r.splits * M * round_up(N, 8) * sizeof(float)) : 0; }
 int run_gemm(GemmP p, const Operand& a, const Operand& b, int dtype, Bump& ws, hipStream_t s) {
-    const Plan r = plan_for(p.M, p.N, p.K, dtype);
+    const Plan r = plan_for(p.M, p.N, p.K, dtype, a.lay == KC);
     p.a = a.p; p.lda = a.ld;
     p.b = b.p; p.ldb = b.ld;
     p.splits = r.splits;
@@ -254,7 +256,7 @@ using namespace insmos::lin;
 
 extern "C" size_t insmos_linear_ws_bytes(int64_t M, int K, int N, int dtype) {
     if (!good_shape(M, K, N, dtype) || !M) return 0;
-    return packed_bytes(M, K, dtype) + packed_bytes(K, N, dtype) + packed_bytes(N, K, dtype) + plan_bytes(plan_for((int)M, N, K, dtype), (int)M, N);
+    return packed_bytes(M, K, dtype) + packed_bytes(K, N, dtype) + packed_bytes(N, K, dtype) + plan_bytes(plan_for((int)M, N, K, dtype, true), (int)M, N);
 }
 extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, const void* bias, const void* residual,
                              int64_t ld_res, int residual_first, int act, int64_t M, int K, int N, int dtype, void* y, int64_t ld_y, void* z,
@@ -269,8 +271,9 @@ extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t
     const hipStream_t s = (hipStream_t)stream;
     Bump bump(ws, ws ? ws_bytes : 0);
     Operand a, b;
-    int rc = operand(x, ld_x, M, K, KC, dtype, bump, s, &a);
-    if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, KC, dtype, bump, s, &b) : operand(w, ld_w, K, N, NC, dtype, bump, s, &b);
+    const bool any = plan_for((int)M, N, K, dtype, true).tile == FEW;
+    int rc = operand(x, ld_x, M, K, KC, dtype, any, bump, s, &a);
+    if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, KC, dtype, any, bump, s, &b) : operand(w, ld_w, K, N, NC, dtype, any, bump, s, &b);
     if (rc != INSMOS_OK) return rc;
     GemmP p = {};
     p.M = (int)M; p.N = N; p.K = K;
@@ -285,7 +288,7 @@ extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t
 extern "C" size_t insmos_linear_backward_ws_bytes(int64_t M, int K, int N, int dtype) {
     if (!good_shape(M, K, N, dtype) || !M) return 0;
     const SlopePlan r = slope_plan(M, N, dtype);
-    const Plan dx = plan_for((int)M, K, N, dtype), dw = plan_for(K, N, (int)M, dtype), dwt = plan_for(N, K, (int)M, dtype);
+    const Plan dx = plan_for((int)M, K, N, dtype, true), dw = plan_for(K, N, (int)M, dtype, false), dwt = plan_for(N, K, (int)M, dtype, false);
     const size_t w1 = plan_bytes(dw, K, N), w2 = plan_bytes(dwt, N, K);
     return packed_bytes(M, N, dtype) + pad256((size_t)r.blocks * N * sizeof(float)) + packed_bytes(K, N, dtype) + packed_bytes(N, K, dtype) +
            packed_bytes(M, K, dtype) + plan_bytes(dx, (int)M, K) + (w1 > w2 ? w1 : w2);
@@ -335,8 +338,9 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
     if (dx) {   // (M, K) = dz (M, N) W^T: k of this product is N
         Operand a, b;
         const int np = round_up(N, (int)chunk);
-        rc = operand(d, ld_d, M, own ? np : N, KC, dtype, bump, s, &a);   // (own rows end in zeros: N may count as padded there)
-        if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, NC, dtype, bump, s, &b) : operand(w, ld_w, K, N, KC, dtype, bump, s, &b);
+        const bool any = plan_for((int)M, K, N, dtype, true).tile == FEW;
+        rc = operand(d, ld_d, M, own ? np : N, KC, dtype, any, bump, s, &a);   // (own rows end in zeros: N may count as padded there)
+        if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, NC, dtype, any, bump, s, &b) : operand(w, ld_w, K, N, KC, dtype, any, bump, s, &b);
         if (rc != INSMOS_OK) return rc;
         GemmP p = {};
         p.M = (int)M; p.N = K; p.K = N;
@@ -346,8 +350,8 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
     }
     if (dw) {   // (K, N) = x^T dz, or its transpose for a (N, K) weight: k of this product is M
         Operand a, b;
-        rc = operand(x, ld_x, M, K, NC, dtype, bump, s, &a);
-        if (rc == INSMOS_OK) rc = operand(d, ld_d, M, N, NC, dtype, bump, s, &b);
+        rc = operand(x, ld_x, M, K, NC, dtype, false, bump, s, &a);
+        if (rc == INSMOS_OK) rc = operand(d, ld_d, M, N, NC, dtype, false, bump, s, &b);
         if (rc != INSMOS_OK) return rc;
         GemmP p = {};
         p.M = w_out_in ? N : K; p.N = w_out_in ? K : N; p.K = (int)M;
