@@ -852,11 +852,13 @@ int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dt
  *   z = x W + bias (+ residual if residual_first);   y = act(z) (+ residual if !residual_first)
  * x (M, K), row pitch ld_x; W (K, N) with row pitch ld_w, or given as (N, K) rows with w_out_in; bias (N) or NULL; residual (M, N), any row
  * pitch >= 0 (0: one row for all), or NULL; y (M, N).  All of one dtype (INSMOS_F32 / BF16 / F16), pitches in elements (at most 2^20, as are
- * K and N); sums in fp32, one rounding per output.  z: receives the value before the activation, or NULL.  Addresses and pitches need only
- * the elements' alignment; operands that are not 16-byte aligned are laid out again in ws.
+ * K and N); sums in fp32, one rounding per output.  Addresses and pitches need only the elements' alignment; operands that are not 16-byte
+ * aligned are laid out again in ws.  slope: NULL, or receives act'(z) for the backward pass, in fp32 for INSMOS_F32 and otherwise as 16 bits
+ * (steps of 2^-15 from -1/2; 0xFFFF: not a number), 16-byte aligned, ld_slope a multiple of 16 bytes that holds N rounded up to 16 bytes; not
+ * without an activation.
  * Backward: dz = dy act'(z);  dx = dz W^T;  dw = x^T dz in the weight's layout;  db = column sums of dz (before its rounding to the type).
- * z: as stored by the forward, for INSMOS_ACT_RELU the values y before a residual or z itself (only their sign counts); unused without an
- * activation.  Each of dx, dw, db, dz may be NULL; dz: 16-byte aligned, ld_dz a multiple of 16 bytes that holds N rounded up to 16 bytes.
+ * slope_kind: INSMOS_SLOPE_NONE (no activation), INSMOS_SLOPE_SIGN (slope holds y = relu(z), of which the sign counts) or INSMOS_SLOPE_STORED.
+ * Each of dx, dw, db, dz may be NULL; dz: 16-byte aligned rows like slope's.
  * ws: 16-byte aligned, insmos_linear*_ws_bytes bytes.  M = 0 is no work for insmos_linear and refused by the backward.
  * ---------------------------------------------------------------------------------------------- */
 #define INSMOS_ACT_NONE 0
@@ -864,13 +866,16 @@ int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dt
 #define INSMOS_ACT_GELU 2      /* z (1 + erf(z / sqrt 2)) / 2 */
 #define INSMOS_ACT_GELU_TANH 3 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
 #define INSMOS_ACT_SILU 4      /* z / (1 + exp(-z)) */
+#define INSMOS_SLOPE_NONE 0
+#define INSMOS_SLOPE_SIGN 1
+#define INSMOS_SLOPE_STORED 2
 size_t insmos_linear_ws_bytes(int64_t M, int K, int N, int dtype);
 int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, const void* bias, const void* residual,
-                  int64_t ld_res, int residual_first, int act, int64_t M, int K, int N, int dtype, void* y, int64_t ld_y, void* z,
-                  int64_t ld_z, void* ws, size_t ws_bytes, void* stream);
+                  int64_t ld_res, int residual_first, int act, int64_t M, int K, int N, int dtype, void* y, int64_t ld_y,
+                  void* slope, int64_t ld_slope, void* ws, size_t ws_bytes, void* stream);
 size_t insmos_linear_backward_ws_bytes(int64_t M, int K, int N, int dtype);
-int insmos_linear_backward(const void* dy, int64_t ld_dy, const void* z, int64_t ld_z, const void* x, int64_t ld_x, const void* w,
-                           int64_t ld_w, int w_out_in, int act, int64_t M, int K, int N, int dtype, void* dx, int64_t ld_dx, void* dw,
+int insmos_linear_backward(const void* dy, int64_t ld_dy, const void* slope, int64_t ld_slope, int slope_kind, const void* x, int64_t ld_x,
+                           const void* w, int64_t ld_w, int w_out_in, int64_t M, int K, int N, int dtype, void* dx, int64_t ld_dx, void* dw,
                            int64_t ld_dw, void* db, void* dz, int64_t ld_dz, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -504,26 +504,26 @@ def _host():
 
 
 class LinearFunction(torch.autograd.Function):
-    """act(x W + b [+ r]) [+ r] with its gradients.  The backward keeps x, W and, for the activation's slope, z rounded to the type (y itself
-    for relu, whose slope is its sign)."""
+    """act(x W + b [+ r]) [+ r] with its gradients.  The backward keeps x, W and the activation's slopes (16 bits each with 16-bit types; y
+    itself for relu, whose slope is its sign)."""
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, residual_first):
         # relu: y > 0 says what z > 0 does, unless a residual was added behind it
         of_y = act == 1 and (residual is None or residual_first)
-        y, z = _host().linear_forward(x, weight, bias, residual, act, residual_first, act != 0 and not of_y)
-        ctx.save_for_backward(x, weight, y if of_y else z)
-        ctx.meta = (act, residual_first, bias is not None, residual is not None)
+        y, slope = _host().linear_forward(x, weight, bias, residual, act, residual_first, act != 0 and not of_y)
+        ctx.save_for_backward(x, weight, y if of_y else slope)
+        ctx.meta = (0 if act == 0 else 1 if of_y else 2, residual_first, bias is not None, residual is not None)   # INSMOS_SLOPE_*
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, z = ctx.saved_tensors
-        act, first, has_bias, has_res = ctx.meta
+        x, weight, slope = ctx.saved_tensors
+        kind, first, has_bias, has_res = ctx.meta
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         need_r = need_r and has_res
-        dx, dw, db, dz = _host().linear_backward(dy, z, x, weight, act, need_x, need_w, need_b and has_bias, need_r and first and act != 0)
+        dx, dw, db, dz = _host().linear_backward(dy, slope, x, weight, kind, need_x, need_w, need_b and has_bias, need_r and first and kind != 0)
         return dx, dw, db, (dz if dz is not None else dy) if need_r else None, None, None
 
 
@@ -535,7 +535,7 @@ def linear(x, weight, bias=None, residual=None, activation=None, residual_first=
     .t()) is read as it lies.  bias (cout,).  residual: the output's shape (an expanded one works: rows of pitch 0).  activation: None,
     "relu", "gelu" (erf), "gelu_tanh" or "silu".  All tensors of one dtype -- float32, bfloat16 or float16 -- on one GPU; sums in fp32.
     Widths up to 2^20.  Differentiable once in all four tensors; without gradients nothing is kept for a backward pass.  In 16 bits the
-    backward rounds z (for the slope) and dz (for the products) once each."""
+    backward rounds dz once, for the products."""
     try:
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):

@@ -219,7 +219,7 @@ int64_t padded(int64_t cols, const at::Tensor& like) {
     return (cols + chunk - 1) / chunk * chunk;
 }
 
-// linear_forward(x, weight, bias or None, residual or None, act, residual_first, keep_z) -> (y, z or None)
+// linear_forward(x, weight, bias or None, residual or None, act, residual_first, keep) -> (y, slopes for the backward pass or None)
 PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         if (n_args != 7 || !g_linear) refuse("internal call");
@@ -254,9 +254,9 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         }
         if (x.numel() / cin > 0x7FFFFF00) refuse("at most " + std::to_string(0x7FFFFF00) + " rows");
         c10::DeviceGuard guard(x.device());
-        at::Tensor y = at::empty(out, x.options().requires_grad(false)), z;
-        const int64_t n = x.numel() / cin, ld_z = padded(cout, x);
-        if (keep) z = at::empty({n, ld_z}, x.options().requires_grad(false));
+        at::Tensor y = at::empty(out, x.options().requires_grad(false)), slope;
+        const int64_t n = x.numel() / cin, ld = padded(cout, x);
+        if (keep) slope = at::empty({n, ld}, x.options().dtype(dt == INSMOS_F32 ? at::kFloat : at::kShort).requires_grad(false));
         if (n && cout) {
             const Rows xr = rows_of(x, cin);
             const Weight wt = weight_of(w);
@@ -265,22 +265,23 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             const size_t need = g_linear_ws(n, (int)cin, (int)cout, dt);
             const at::Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
             checked(g_linear(xr.t.data_ptr(), xr.ld, wt.t.data_ptr(), wt.ld, wt.out_in, at_ptr(b), at_ptr(rr.t), rr.ld, first, act, n, (int)cin, (int)cout,
-                             dt, y.data_ptr(), cout, at_ptr(z), ld_z, at_ptr(ws), need, stream_of(x)), "insmos_linear");
+                             dt, y.data_ptr(), cout, at_ptr(slope), ld, at_ptr(ws), need, stream_of(x)), "insmos_linear");
         }
-        return Py_BuildValue("NN", wrap(y), wrap(z));
+        return Py_BuildValue("NN", wrap(y), wrap(slope));
     });
 }
-// linear_backward(dy, z or None, x, weight, act, need_x, need_w, need_b, need_dz) -> (dx, dweight, dbias, dz), None where not needed
+// linear_backward(dy, slopes (or y) or None, x, weight, INSMOS_SLOPE_*, need_x, need_w, need_b, need_dz) -> (dx, dweight, dbias, dz), None
+// where not needed
 PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         if (n_args != 9 || !g_backward) refuse("internal call");
         const at::Tensor &dy = arg(a[0], "the gradient"), &x = arg(a[2], "x"), &w = arg(a[3], "weight");
-        at::Tensor z;
-        if (a[1] != Py_None) z = arg(a[1], "z");
-        const int act = (int)PyLong_AsLong(a[4]);
+        at::Tensor slope;
+        if (a[1] != Py_None) slope = arg(a[1], "slope");
+        const int kind = (int)PyLong_AsLong(a[4]);
         const bool need_x = PyObject_IsTrue(a[5]), need_w = PyObject_IsTrue(a[6]), need_b = PyObject_IsTrue(a[7]), need_dz = PyObject_IsTrue(a[8]);
         const int dt = dtype_code(x.scalar_type());
-        const int64_t cin = w.size(0), cout = w.size(1), n = x.numel() / cin, ld_z = padded(cout, x);
+        const int64_t cin = w.size(0), cout = w.size(1), n = x.numel() / cin, ld = padded(cout, x);
         if (dy.scalar_type() != x.scalar_type() || dy.device() != x.device()) refuse("the gradient is of another type or device than the output");
         c10::DeviceGuard guard(x.device());
         const auto opt = x.options().requires_grad(false);
@@ -290,14 +291,14 @@ PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         if (need_w) dw = wt.out_in ? at::empty({cout, cin}, opt) : at::empty({cin, cout}, opt);
         if (need_b) db = at::empty({cout}, opt);
         if (n && cout) {
-            if (need_dz) dz = at::empty({n, ld_z}, opt);
+            if (need_dz) dz = at::empty({n, ld}, opt);
             if (need_x || need_w || need_b || need_dz) {
                 const Rows d = rows_of(dy, cout), xr = rows_of(x, cin);
                 const size_t need = g_backward_ws(n, (int)cin, (int)cout, dt);
                 const at::Tensor ws = at::empty({(int64_t)need}, opt.dtype(at::kByte));
-                checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(z), z.defined() ? (z.dim() == 2 && z.size(1) == ld_z ? ld_z : cout) : 0, xr.t.data_ptr(), xr.ld,
-                                   wt.t.data_ptr(), wt.ld, wt.out_in, act, n, (int)cin, (int)cout, dt, at_ptr(dx), cin, at_ptr(dw),
-                                   wt.out_in ? cin : cout, at_ptr(db), at_ptr(dz), ld_z, ws.data_ptr(), need, stream_of(x)),
+                checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(slope), kind == INSMOS_SLOPE_STORED ? ld : cout, kind, xr.t.data_ptr(), xr.ld,
+                                   wt.t.data_ptr(), wt.ld, wt.out_in, n, (int)cin, (int)cout, dt, at_ptr(dx), cin, at_ptr(dw),
+                                   wt.out_in ? cin : cout, at_ptr(db), at_ptr(dz), ld, ws.data_ptr(), need, stream_of(x)),
                         "insmos_linear_backward");
             }
             if (need_dz) dz = dz.narrow(1, 0, cout).reshape(dy.sizes());

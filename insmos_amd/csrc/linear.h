@@ -36,7 +36,7 @@ template <> struct Mem8<__bf16> { typedef __bf16 t __attribute__((ext_vector_typ
 template <> struct Mem8<_Float16> { typedef _Float16 t __attribute__((ext_vector_type(8), aligned(2))); };
 
 enum { KC = 0, NC = 1 };                                            // which index of an operand is contiguous
-enum { T256 = 0, T128 = 1, TNARROW = 2, TFLAT = 3, FEW = 4 };       // tiles 256x256, 128x128, 128x32 (few columns), 32x128 (few rows); k_linear_few
+enum { T256 = 0, T128, T128X64, T64X128, T128X32, T32X128, FEW };   // tiles (rows x columns); k_linear_few
 
 struct GemmP {
     const void* a;
@@ -52,8 +52,8 @@ struct GemmP {
     int64_t ld_res;
     void* y;
     int64_t ld_y;
-    void* z;              // the value before the activation, or null
-    int64_t ld_z;
+    void* slope;          // act'(z) for the backward pass (see Slope), or null
+    int64_t ld_slope;     // a multiple of 16 bytes
     int act, res_first;
 };
 
@@ -76,34 +76,37 @@ __device__ __forceinline__ float normal_tail(float z, float& e) {
     e = __expf(-0.5f * z * z);
     return p * t * e;
 }
-// act != INSMOS_ACT_NONE.  z times a weight between 0 and 1; silu's and the tanh form's are sigmoids: (1 + tanh u) / 2 = sigmoid(2 u).  (One formula for both: the
-// epilogue's code is part of every tile's time when it has to be fetched.)
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == INSMOS_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+// act(z) and act'(z), act != INSMOS_ACT_NONE.  z times a weight between 0 and 1; silu's and the tanh form's are sigmoids: (1 + tanh u) / 2 =
+// sigmoid(2 u).  (One formula for both: the epilogue's code is part of every tile's time when it has to be fetched.)
+__device__ __forceinline__ float activate(float z, int act, float& slope) {
+    if (act == INSMOS_ACT_RELU) {
+        slope = z > 0.f ? 1.f : (z != z ? z : 0.f);
+        return z > 0.f ? z : (z != z ? z : 0.f);
+    }
     if (act == INSMOS_ACT_GELU) {
         float e;
-        const float tail = normal_tail(z, e);
-        return z * (z > 0.f ? 1.f - tail : tail);
+        const float tail = normal_tail(z, e), phi = z > 0.f ? 1.f - tail : tail;
+        slope = phi + z * e * 0.3989422804014327f;
+        return z * phi;
     }
     const float c0 = act == INSMOS_ACT_SILU ? 1.f : 2.f * kGelu0, c1 = act == INSMOS_ACT_SILU ? 0.f : 2.f * kGelu0 * kGelu1;
-    return z * sigmoid(z * (c0 + c1 * (z * z)));
+    const float z2 = z * z, s = sigmoid(z * (c0 + c1 * z2)), y = z * s;
+    slope = s + y * (1.f - s) * (c0 + 3.f * c1 * z2);
+    return y;
 }
-__device__ __forceinline__ float slope(float z, int act) {
-    switch (act) {
-        case INSMOS_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-        case INSMOS_ACT_GELU: {
-            float e;
-            const float tail = normal_tail(z, e);
-            return (z > 0.f ? 1.f - tail : tail) + z * e * 0.3989422804014327f;
-        }
-        case INSMOS_ACT_GELU_TANH: {
-            const float s = sigmoid(2.f * kGelu0 * (z + kGelu1 * z * z * z));
-            return s + z * 2.f * s * (1.f - s) * kGelu0 * (1.f + 3.f * kGelu1 * z * z);
-        }
-        case INSMOS_ACT_SILU: { const float s = sigmoid(z); return s * (1.f + z * (1.f - s)); }
-    }
-    return 1.f;
-}
+// What the backward pass is given of act'(z): the value itself in fp32; with 16-bit types 16 bits of it in steps of 2^-15 from -1/2 on (all
+// slopes lie in -0.13 .. 1.13), 0xFFFF where it is none.  A z rounded to the type would cost the same bytes and ten times the error (fp16), and
+// the backward would have to compute the slope again.
+template <class T> struct Slope {
+    typedef uint16_t t;
+    static __device__ __forceinline__ uint16_t store(float s) { return s == s ? (uint16_t)(int)rintf(fminf(fmaxf(s + 0.5f, 0.f), 1.99f) * 32768.f) : (uint16_t)0xFFFF; }
+    static __device__ __forceinline__ float load(uint16_t c) { return c == 0xFFFF ? __builtin_nanf("") : (float)c * 0x1p-15f - 0.5f; }
+};
+template <> struct Slope<float> {
+    typedef float t;
+    static __device__ __forceinline__ float store(float s) { return s; }
+    static __device__ __forceinline__ float load(float s) { return s; }
+};
 template <class T>
 __device__ __forceinline__ f32x8 load8(const void* q, int64_t i) { return __builtin_convertvector(*(const typename Mem8<T>::t*)((const T*)q + i), f32x8); }
 template <class T>
@@ -116,10 +119,20 @@ template <class T>
 __device__ __forceinline__ void epilogue8(const GemmP& p, int m, int n, f32x8 v, f32x8 b, f32x8 r) {
     v += b;
     if (p.res_first) v += r;
-    if (p.z) store8<T>(p.z, m * p.ld_z + n, v);
-    if (p.act) {
+    float s;
+    if (p.slope) {   // (with an activation only)
+        typedef typename Slope<T>::t S;
+        typedef S S8 __attribute__((ext_vector_type(8), aligned(16)));
+        S8 c;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = activate(v[e], p.act);
+        for (int e = 0; e < 8; ++e) {
+            v[e] = activate(v[e], p.act, s);
+            c[e] = Slope<T>::store(s);
+        }
+        *(S8*)((S*)p.slope + m * p.ld_slope + n) = c;
+    } else if (p.act) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = activate(v[e], p.act, s);
     }
     if (!p.res_first) v += r;
     store8<T>(p.y, m * p.ld_y + n, v);
@@ -134,8 +147,9 @@ __device__ __forceinline__ void epilogue1(const GemmP& p, int m, int n, f32x8 v)
         if (p.bias) u += (float)((const T*)p.bias)[n + e];
         const float r = p.res ? (float)((const T*)p.res)[m * p.ld_res + n + e] : 0.f;
         if (p.res_first) u += r;
-        if (p.z) ((T*)p.z)[m * p.ld_z + n + e] = (T)u;
-        if (p.act) u = activate(u, p.act);
+        float s = 1.f;
+        if (p.act) u = activate(u, p.act, s);
+        if (p.slope) ((typename Slope<T>::t*)p.slope)[m * p.ld_slope + n + e] = Slope<T>::store(s);
         if (!p.res_first) u += r;
         ((T*)p.y)[m * p.ld_y + n + e] = (T)u;
     }
@@ -326,6 +340,7 @@ struct Gemm {
     // lines of C, and in a loop: unrolled over the sums' registers, the code alone cost some 10 us per launch and 4 us per tile.
     static __device__ __forceinline__ void finish(LIN_LDS char* __restrict l, LIN_LDS char* __restrict turn, const GemmP& p, const Item& it, bool more,
                                                   const Item& next, TA& ta, TB& tb, const f32x16 (&acc)[TM][TN], int wave, int lane) {
+        static_assert(NW * TN * 4096 <= SA + SB, "`turn` is one tile buffer");
         if (more) fill(l, p, next, ta, tb, wave, lane);
         constexpr int CH = TN * 8, LPR = TN * 4, RPP = 64 / LPR, PASSES = 32 / RPP;   // chunks and lanes per row, rows per pass
         typedef typename Mem8<T>::t M8;
@@ -651,12 +666,15 @@ int launch_gemm_l(const GemmP& p, int tile, hipStream_t s) {
             return INSMOS_OK;
         }
     }
+    // persistent: as many workgroups as fit on the CUs at once
     if constexpr (sizeof(T) == 2) {
-        if (tile == T256) rc = launch_tile<T, LA, LB, 256, 256, 2, 4>(p, 256, s);   // one workgroup per CU, walking its items
+        if (tile == T256) rc = launch_tile<T, LA, LB, 256, 256, 2, 4>(p, 256, s);
     }
-    if (tile == T128) rc = launch_tile<T, LA, LB, 128, 128, 2, 2>(p, 512, s);   // two per CU
-    if (tile == TNARROW) rc = launch_tile<T, LA, LB, 128, 32, 4, 1>(p, 1024, s);   // four
-    if (tile == TFLAT) rc = launch_tile<T, LA, LB, 32, 128, 1, 4>(p, 1024, s);
+    if (tile == T128) rc = launch_tile<T, LA, LB, 128, 128, 2, 2>(p, 512, s);
+    if (tile == T128X64) rc = launch_tile<T, LA, LB, 128, 64, 2, 2>(p, 768, s);
+    if (tile == T64X128) rc = launch_tile<T, LA, LB, 64, 128, 1, 4>(p, 768, s);
+    if (tile == T128X32) rc = launch_tile<T, LA, LB, 128, 32, 4, 1>(p, 1024, s);
+    if (tile == T32X128) rc = launch_tile<T, LA, LB, 32, 128, 1, 4>(p, 1024, s);
     if (rc != INSMOS_OK || p.splits == 1) return rc;
     const int64_t rows8 = (int64_t)p.M * (p.ld_part / 8);
     // many parts are few results: 16 lanes each (469 parts of 64 x 128 fp32: 129 -> 9 us)

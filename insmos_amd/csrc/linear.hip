@@ -62,34 +62,44 @@ int operand(const void* p, int64_t ld, int64_t rows, int cols, int lay, int dtyp
 
 // ---- tile and parts ---------------------------------------------------------------------------------------------------------
 struct Plan { int tile, splits; };
-// Rates of a full chip: 256x256 tiles 1200 TFLOP/s (bf16, one workgroup per CU), 128x128 1050 (two per CU); a launch takes as long as its fullest
-// CU, so the larger tile pays only where its tiles fill whole rounds of 256.  Up to 32 rows or columns the flat tiles waste least.
-// Where the tiles leave CUs idle, k is cut into parts, each at least 4 k tiles long, until about two workgroups per CU are there.
+// Up to 32 rows (x W alone) there is a kernel of its own.  Otherwise the tile and the number of parts of k with the shortest predicted time:
+//   rounds of the workgroups that fit on the chip, each k tiles x max(0.75 us, workgroups per CU x a tile's work at the CU's rate) + a fixed
+//   part for its first loads and its epilogue; with parts, their bytes at 4 TB/s and another launch.
+// Rates (all CUs together, TFLOP/s) and fixed parts (us) are measured; predicted / measured, us, bf16: 8192 x 1024 x 1024 128x128 24 / 24,
+// 256x256 34 / 32; 2048^3 128x64 29 / 26, 128x128 32 / 31; 512 x 4096 x 512 128x64 in 8 parts 18 / 15, 128x128 in 16 23 / 21; fp32:
+// 300000 x 128 x 256 128x128 234 / 231, 128x64 212 / 213; 119817 x 64 x 128 128x128 31 / 37, 128x32 29 / 33.
 Plan plan_for(int M, int N, int K, int dtype, bool xw) {   // xw: the first operand has contiguous k
     const int bk = 128 / (int)size_of(dtype), nk = (K + bk - 1) / bk;
-    Plan r = {T128, 1};
-    int64_t tiles, want = 512;
-    const int64_t t128 = (int64_t)((M + 127) / 128) * ((N + 127) / 128), t256 = (int64_t)((M + 255) / 256) * ((N + 255) / 256);
     // (one workgroup per 32 columns walks all of k: 16 x 8192 x 256 takes 25 us that way and 10 in parts)
-    if (M <= 32 && xw && (K <= 4096 || N >= 4096)) { r.tile = FEW; return r; }
-    if (M <= 32) { r.tile = TFLAT; tiles = (N + 127) / 128; want = 1024; }
-    else if (N <= 32) { r.tile = TNARROW; tiles = (M + 127) / 128; want = 1024; }
-    else {
-        tiles = t128;
-        if (dtype != INSMOS_F32) {
-            const double c256 = (double)((t256 + 255) / 256) * 4 / 1200, c128 = (double)((t128 + 511) / 512) * 2 / 1050;
-            if (c256 <= c128) { r.tile = T256; tiles = t256; want = 256; }
+    if (M <= 32 && xw && (K <= 4096 || N >= 4096)) return {FEW, 1};
+    struct Shape { int tile, bm, bn, slots; double rate, rate32, fixed; };
+    static const Shape shapes[] = {{T256, 256, 256, 256, 1250, 0, 6},     {T128, 128, 128, 512, 1050, 140, 8},    {T128X64, 128, 64, 768, 800, 135, 5},
+                                   {T64X128, 64, 128, 768, 800, 135, 5},  {T128X32, 128, 32, 1024, 500, 120, 3}, {T32X128, 32, 128, 1024, 500, 120, 3}};
+    static const int parts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512, 768, 1024};
+    Plan best = {T128, 1};
+    double least = 1e300;
+    for (const Shape& c : shapes) {
+        const double rate = dtype == INSMOS_F32 ? c.rate32 : c.rate;
+        if (rate == 0) continue;
+        const int64_t tiles = (int64_t)((M + c.bm - 1) / c.bm) * ((N + c.bn - 1) / c.bn);
+        const double unit = 2.0 * c.bm * c.bn * bk * 256 / rate * 1e-6;   // us of a k tile on one CU
+        for (int want : parts) {
+            if (want > 1 && (tiles * want > c.slots || nk / want < 2)) break;
+            const int per = (nk + want - 1) / want, splits = (nk + per - 1) / per;   // no part without work
+            const int64_t items = tiles * splits, full = items / c.slots, rest = items % c.slots;
+            auto round = [&](int64_t n) {   // n workgroups at once
+                const double busy = (double)((n + 255) / 256) * unit;
+                return per * (busy > 0.75 ? busy : 0.75) + c.fixed;
+            };
+            double t = full * round(c.slots) + (rest ? round(rest) : 0);
+            if (splits > 1) t += (double)splits * M * N * 8 / 4e6 + 3;
+            if (t < least) {
+                least = t;
+                best = {c.tile, splits};
+            }
         }
     }
-    if (tiles * 2 <= want) {
-        int64_t s = want / tiles;
-        if (s > nk / 4) s = nk / 4;
-        if (s > 1) {
-            const int per = (int)((nk + s - 1) / s);
-            r.splits = (nk + per - 1) / per;   // no part without work
-        }
-    }
-    return r;
+    return best;
 }
 size_t plan_bytes(const Plan& r, int M, int N) { return r.splits > 1 ? pad256((size_t)r.splits * M * round_up(N, 8) * sizeof(float)) : 0; }
 int run_gemm(GemmP p, const Operand& a, const Operand& b, int dtype, Bump& ws, hipStream_t s) {
@@ -109,67 +119,71 @@ int run_gemm(GemmP p, const Operand& a, const Operand& b, int dtype, Bump& ws, h
 // ---- dz and the column sums -------------------------------------------------------------------------------------------------
 struct SlopeP {
     const void* dy;
-    const void* z;       // z, or y for relu; null: no activation
+    const void* slope;   // INSMOS_SLOPE_SIGN: y; INSMOS_SLOPE_STORED: what the forward stored
     void* dz;            // or null: column sums alone
     float* part;         // [row blocks][ld_part] or null
-    int64_t ld_dy, ld_z, ld_dz;
+    int64_t ld_dy, ld_slope, ld_dz;
     int64_t M;
-    int N, ld_part, act, rows;   // rows per workgroup
+    int N, ld_part, kind, rows;   // rows per workgroup
     int lanes;           // column lanes (a power of two <= 32)
 };
 // 256 lanes = `lanes` over the columns (16 bytes each) x the rest over rows; dz rounds dy act'(z) once to the type (the products read it in that
 // type); the column sums are taken before the rounding, in fp32, rows in a fixed order.
-template <class T>
+template <class T, int KIND>
 __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 16 / sizeof(T), U = 4;   // columns per lane, rows in flight
     typedef T TV __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));   // (16 bytes at any address)
+    typedef typename Slope<T>::t S;
+    typedef S SV __attribute__((ext_vector_type(16 / sizeof(T))));
     const int lanes = p.lanes, rl = 256 / lanes, cl = threadIdx.x % lanes, r0 = threadIdx.x / lanes;
     const int n = (blockIdx.x * lanes + cl) * V;
     const int64_t from = (int64_t)blockIdx.y * p.rows, to = min(p.M, from + p.rows);
     float sum[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) sum[e] = 0.f;
-    auto row = [&](int64_t m, const float (&d0)[V], const float (&zz)[V]) {
-        TV out;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            float d = d0[e];
-            if (p.act && n + e < p.N) d *= slope(zz[e], p.act);
-            sum[e] += d;
-            out[e] = (T)d;
-        }
-        if (p.dz) *(TV*)((T*)p.dz + m * p.ld_dz + n) = out;   // (dz rows are padded to whole chunks, with zeros)
-    };
-    if (n + V <= p.N) {
-        constexpr int U = 4;   // rows in flight
+    if (n < p.N) {
+        const bool whole = n + V <= p.N;
         for (int64_t m = from + r0; m < to; m += U * rl) {
-            TV a[U], b[U];
+            TV a[U], y[U];
+            SV c[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int64_t q = min(m + u * rl, to - 1);
-                a[u] = *(const TV*)((const T*)p.dy + q * p.ld_dy + n);
-                b[u] = p.z ? *(const TV*)((const T*)p.z + q * p.ld_z + n) : a[u];
+                const T* dy = (const T*)p.dy + q * p.ld_dy + n;
+                if (whole) a[u] = *(const TV*)dy;
+                else
+#pragma unroll
+                    for (int e = 0; e < V; ++e) a[u][e] = n + e < p.N ? dy[e] : (T)0.f;
+                if (KIND == INSMOS_SLOPE_STORED) c[u] = *(const SV*)((const S*)p.slope + q * p.ld_slope + n);   // (rows of whole chunks)
+                if (KIND == INSMOS_SLOPE_SIGN) {
+                    const T* yy = (const T*)p.slope + q * p.ld_slope + n;
+                    if (whole) y[u] = *(const TV*)yy;
+                    else
+#pragma unroll
+                        for (int e = 0; e < V; ++e) y[u][e] = n + e < p.N ? yy[e] : (T)0.f;
+                }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (m + u * rl >= to) break;
-                float d[V], zz[V];
+                typedef T AV __attribute__((ext_vector_type(16 / sizeof(T))));
+                AV out;
 #pragma unroll
-                for (int e = 0; e < V; ++e) { d[e] = (float)a[u][e]; zz[e] = (float)b[u][e]; }
-                row(m + u * rl, d, zz);
+                for (int e = 0; e < V; ++e) {
+                    float d = (float)a[u][e];
+                    if (KIND == INSMOS_SLOPE_STORED && n + e < p.N) {
+                        const float v = Slope<T>::load(c[u][e]);
+                        d = v == 0.f ? 0.f : d * v;   // (where a relu is shut, whatever comes from behind stays there)
+                    }
+                    if (KIND == INSMOS_SLOPE_SIGN) {
+                        const float v = (float)y[u][e];
+                        d = v > 0.f ? d : (v != v ? v : 0.f);
+                    }
+                    sum[e] += d;
+                    out[e] = (T)d;
+                }
+                if (p.dz) *(AV*)((T*)p.dz + (m + u * rl) * p.ld_dz + n) = out;   // (dz rows are padded to whole chunks, with zeros)
             }
-        }
-    } else if (n < p.N) {
-        for (int64_t m = from + r0; m < to; m += rl) {
-            const T* dy = (const T*)p.dy + m * p.ld_dy + n;
-            const T* z = p.z ? (const T*)p.z + m * p.ld_z + n : nullptr;
-            float d[V], zz[V];
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                d[e] = n + e < p.N ? (float)dy[e] : 0.f;
-                zz[e] = z && n + e < p.N ? (float)z[e] : 0.f;
-            }
-            row(m, d, zz);
         }
     }
     if (!p.part) return;
@@ -190,22 +204,24 @@ __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {
             if (n + e < p.N) p.part[(int64_t)blockIdx.y * p.ld_part + n + e] = s[threadIdx.x][e];
     }
 }
-// db[n] = sum over the row blocks: 16 lanes per column, then a tree
+// db[n] = sum over the row blocks: 64 lanes per column, then a tree
 template <class T>
-__global__ void __launch_bounds__(256) k_linear_colsum(const float* __restrict__ part, int blocks, int N, int ld, T* __restrict__ db) {
+__global__ void __launch_bounds__(1024) k_linear_colsum(const float* __restrict__ part, int blocks, int N, int ld, T* __restrict__ db) {
     const int n = blockIdx.x * 16 + (threadIdx.x & 15), r = threadIdx.x >> 4;
     float s = 0.f;
-    if (n < N)
-        for (int b = r; b < blocks; b += 16) s += part[(int64_t)b * ld + n];
-    __shared__ float w[16][17];
+    if (n < N) {
+#pragma unroll 4
+        for (int b = r; b < blocks; b += 64) s += part[(int64_t)b * ld + n];
+    }
+    __shared__ float w[64][17];
     w[r][threadIdx.x & 15] = s;
     __syncthreads();
-    if (r == 0 && n < N) {
-        float t = 0.f;
 #pragma unroll
-        for (int q = 0; q < 16; ++q) t += w[q][threadIdx.x & 15];
-        db[n] = (T)t;
+    for (int h = 32; h; h >>= 1) {
+        if (r < h) w[r][threadIdx.x & 15] += w[r + h][threadIdx.x & 15];
+        __syncthreads();
     }
+    if (r == 0 && n < N) db[n] = (T)w[0][threadIdx.x];
 }
 struct SlopePlan { int lanes, strips, rows, blocks; };
 SlopePlan slope_plan(int64_t M, int N, int dtype) {
@@ -227,12 +243,13 @@ SlopePlan slope_plan(int64_t M, int N, int dtype) {
 }
 template <class T>
 int run_slope_t(const SlopeP& p, const SlopePlan& r, void* db, hipStream_t s) {
-    const auto kernel = k_linear_slope<T>;
+    const auto kernel = p.kind == INSMOS_SLOPE_STORED ? k_linear_slope<T, INSMOS_SLOPE_STORED>
+                        : p.kind == INSMOS_SLOPE_SIGN ? k_linear_slope<T, INSMOS_SLOPE_SIGN> : k_linear_slope<T, INSMOS_SLOPE_NONE>;
     INSMOS_LAUNCH(kernel, dim3(r.strips, r.blocks), dim3(256), 0, s, p);
     HIP_TRY(hipGetLastError());
     if (db) {
         const auto sum = k_linear_colsum<T>;
-        INSMOS_LAUNCH(sum, dim3((p.N + 15) / 16), dim3(256), 0, s, (const float*)p.part, r.blocks, p.N, p.ld_part, (T*)db);
+        INSMOS_LAUNCH(sum, dim3((p.N + 15) / 16), dim3(1024), 0, s, (const float*)p.part, r.blocks, p.N, p.ld_part, (T*)db);
         HIP_TRY(hipGetLastError());
     }
     return INSMOS_OK;
@@ -246,7 +263,12 @@ bool good_matrix(const void* p, int64_t ld, int64_t cols, int dtype) {
     return p && ld >= cols && ld <= (int64_t)1 << 20 && (uintptr_t)p % size_of(dtype) == 0;
 }
 // dz needs a buffer of its own where there is an activation or dy cannot be loaded as it is
-bool needs_dz(const void* dy, int64_t ld_dy, int N, int act, int dtype) { return act != INSMOS_ACT_NONE || !loadable(dy, ld_dy, N, KC, dtype); }
+bool needs_dz(const void* dy, int64_t ld_dy, int N, int kind, int dtype) { return kind != INSMOS_SLOPE_NONE || !loadable(dy, ld_dy, N, KC, dtype); }
+// rows of a buffer in the library's own layout: 16-byte aligned, whole chunks
+bool good_rows(const void* p, int64_t ld, int N, int dtype) {
+    const int64_t chunk = 16 / (int64_t)size_of(dtype);
+    return (uintptr_t)p % 16 == 0 && ld % chunk == 0 && ld >= round_up(N, (int)chunk) && ld <= (int64_t)1 << 20;
+}
 }  // namespace
 }  // namespace lin
 }  // namespace insmos
@@ -259,13 +281,13 @@ extern "C" size_t insmos_linear_ws_bytes(int64_t M, int K, int N, int dtype) {
     return packed_bytes(M, K, dtype) + packed_bytes(K, N, dtype) + packed_bytes(N, K, dtype) + plan_bytes(plan_for((int)M, N, K, dtype, true), (int)M, N);
 }
 extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, const void* bias, const void* residual,
-                             int64_t ld_res, int residual_first, int act, int64_t M, int K, int N, int dtype, void* y, int64_t ld_y, void* z,
-                             int64_t ld_z, void* ws, size_t ws_bytes, void* stream) {
+                             int64_t ld_res, int residual_first, int act, int64_t M, int K, int N, int dtype, void* y, int64_t ld_y,
+                             void* slope, int64_t ld_slope, void* ws, size_t ws_bytes, void* stream) {
     if (!good_shape(M, K, N, dtype) || act < INSMOS_ACT_NONE || act > INSMOS_ACT_SILU) return INSMOS_EINVAL;
     if (M == 0) return INSMOS_OK;
     const uintptr_t es = size_of(dtype);
     if (!good_matrix(x, ld_x, K, dtype) || !good_matrix(w, ld_w, w_out_in ? K : N, dtype) || !good_matrix(y, ld_y, N, dtype) ||
-        (z && !good_matrix(z, ld_z, N, dtype)) || (residual && (ld_res < 0 || ld_res > (int64_t)1 << 20 || (uintptr_t)residual % es)) ||
+        (slope && (act == INSMOS_ACT_NONE || !good_rows(slope, ld_slope, N, dtype))) || (residual && (ld_res < 0 || ld_res > (int64_t)1 << 20 || (uintptr_t)residual % es)) ||
         (uintptr_t)bias % es || (uintptr_t)ws % 16)
         return INSMOS_EINVAL;
     const hipStream_t s = (hipStream_t)stream;
@@ -280,7 +302,7 @@ extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t
     p.bias = bias;
     p.res = residual; p.ld_res = ld_res; p.res_first = residual && residual_first;
     p.y = y; p.ld_y = ld_y;
-    p.z = z; p.ld_z = ld_z;
+    p.slope = slope; p.ld_slope = ld_slope;
     p.act = act;
     return run_gemm(p, a, b, dtype, bump, s);
 }
@@ -293,28 +315,29 @@ extern "C" size_t insmos_linear_backward_ws_bytes(int64_t M, int K, int N, int d
     return packed_bytes(M, N, dtype) + pad256((size_t)r.blocks * N * sizeof(float)) + packed_bytes(K, N, dtype) + packed_bytes(N, K, dtype) +
            packed_bytes(M, K, dtype) + plan_bytes(dx, (int)M, K) + (w1 > w2 ? w1 : w2);
 }
-extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void* z, int64_t ld_z, const void* x, int64_t ld_x, const void* w,
-                                      int64_t ld_w, int w_out_in, int act, int64_t M, int K, int N, int dtype, void* dx, int64_t ld_dx, void* dw,
+extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void* slope, int64_t ld_slope, int slope_kind, const void* x,
+                                      int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, int64_t M, int K, int N, int dtype, void* dx, int64_t ld_dx, void* dw,
                                       int64_t ld_dw, void* db, void* dz, int64_t ld_dz, void* ws, size_t ws_bytes, void* stream) {
-    if (!good_shape(M, K, N, dtype) || M < 1 || act < INSMOS_ACT_NONE || act > INSMOS_ACT_SILU) return INSMOS_EINVAL;
+    if (!good_shape(M, K, N, dtype) || M < 1 || slope_kind < INSMOS_SLOPE_NONE || slope_kind > INSMOS_SLOPE_STORED) return INSMOS_EINVAL;
     const int64_t es = size_of(dtype), chunk = 16 / es;
-    if (!good_matrix(dy, ld_dy, N, dtype) || (act && !good_matrix(z, ld_z, N, dtype)) || (dx && !good_matrix(dx, ld_dx, K, dtype)) ||
+    if (!good_matrix(dy, ld_dy, N, dtype) || (slope_kind == INSMOS_SLOPE_SIGN && !good_matrix(slope, ld_slope, N, dtype)) ||
+        (slope_kind == INSMOS_SLOPE_STORED && (!slope || !good_rows(slope, ld_slope, N, dtype))) || (dx && !good_matrix(dx, ld_dx, K, dtype)) ||
         (dx && !good_matrix(w, ld_w, w_out_in ? K : N, dtype)) || (dw && !good_matrix(x, ld_x, K, dtype)) ||
         (dw && !good_matrix(dw, ld_dw, w_out_in ? K : N, dtype)) || (uintptr_t)db % es || (uintptr_t)ws % 16)
         return INSMOS_EINVAL;
     // dz given: it is an output too; rows padded to whole chunks
-    if (dz && ((uintptr_t)dz % 16 || ld_dz % chunk || ld_dz < round_up(N, (int)chunk) || ld_dz > (int64_t)1 << 20)) return INSMOS_EINVAL;
+    if (dz && !good_rows(dz, ld_dz, N, dtype)) return INSMOS_EINVAL;
     const hipStream_t s = (hipStream_t)stream;
     Bump bump(ws, ws ? ws_bytes : 0);
     int rc = INSMOS_OK;
     const void* d = dy;
     int64_t ld_d = ld_dy;
-    const bool own = dz || ((dx || dw) && needs_dz(dy, ld_dy, N, act, dtype));
+    const bool own = dz || ((dx || dw) && needs_dz(dy, ld_dy, N, slope_kind, dtype));
     if (own || db) {
         SlopeP q = {};
         q.dy = dy; q.ld_dy = ld_dy;
-        q.z = act ? z : nullptr; q.ld_z = ld_z;
-        q.act = act;
+        q.slope = slope; q.ld_slope = ld_slope;
+        q.kind = slope_kind;
         q.M = M; q.N = N;
         const SlopePlan r = slope_plan(M, N, dtype);
         q.rows = r.rows;
