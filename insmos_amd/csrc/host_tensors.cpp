@@ -85,7 +85,6 @@ PyObject* opt_table(PyObject*, PyObject* args) {
         const int code = dtype_code(first.scalar_type());
         std::string a, b;
         if (code < 0) throw Refused(std::string(what) + ": float32, bfloat16 or float16, not " + place(first, a));
-        if (!any_device && !first.is_cuda()) throw Refused(std::string(what) + ": tensors on the GPU, not on " + first.device().str());
         Py_ssize_t used = 0;
         int64_t off = 0;
         std::vector<std::pair<uintptr_t, uintptr_t>> spans;
@@ -120,6 +119,7 @@ PyObject* opt_table(PyObject*, PyObject* args) {
         std::sort(spans.begin(), spans.end());
         for (size_t i = 1; i < spans.size(); ++i)
             if (spans[i].first < spans[i - 1].second) throw Refused(std::string(what) + ": two parameters share memory");
+        if (!any_device && !first.is_cuda()) throw Refused(std::string(what) + ": tensors on the GPU, not on " + first.device().str());
         result = Py_BuildValue("niLO", used, code, (long long)off, reorder);
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
@@ -228,7 +228,6 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         const int dt = dtype_code(x.scalar_type());
         std::string buf;
         if (dt < 0) refuse(std::string("float32, bfloat16 or float16, not ") + place(x, buf));
-        if (!x.is_cuda()) refuse("tensors on the GPU, not on " + x.device().str());
         if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(0)) refuse("x (..., cin) and weight (cin, cout), not " + shape(x) + " and " + shape(w));
         const int64_t cin = w.size(0), cout = w.size(1);
         if (cin < 1 || cin > kMost || cout > kMost) refuse("widths from 1 to 2^20, not " + std::to_string(cin) + " -> " + std::to_string(cout));
@@ -253,6 +252,7 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             if (r.sizes() != at::IntArrayRef(out)) refuse("residual of the output's shape, not " + shape(r));
         }
         if (x.numel() / cin > 0x7FFFFF00) refuse("at most " + std::to_string(0x7FFFFF00) + " rows");
+        if (!x.is_cuda()) refuse("tensors on the GPU, not on " + x.device().str());
         c10::DeviceGuard guard(x.device());
         at::Tensor y = at::empty(out, x.options().requires_grad(false)), slope;
         const int64_t n = x.numel() / cin, ld = padded(cout, x);

@@ -90,7 +90,8 @@ __device__ __forceinline__ float activate(float z, int act, float& slope) {
         return z * phi;
     }
     const float c0 = act == INSMOS_ACT_SILU ? 1.f : 2.f * kGelu0, c1 = act == INSMOS_ACT_SILU ? 0.f : 2.f * kGelu0 * kGelu1;
-    const float z2 = z * z, s = sigmoid(z * (c0 + c1 * z2)), y = z * s;
+    const float z2 = fminf(z * z, 3e38f);   // (c1 = 0 times inf would be none)
+    const float s = sigmoid(z * (c0 + c1 * z2)), y = z * s;
     slope = s + y * (1.f - s) * (c0 + 3.f * c1 * z2);
     return y;
 }

@@ -346,6 +346,14 @@ class InsMOSTrainer:
         self._reducer = BucketedGradReducer(self.params, bucket_bytes, overlap=overlap, force_collective=force_collective)
         return self._reducer
 
+    def make_optimizer(self, **options):
+        """The reference's optimiser (models/models.py:185-190: Adam, weight decay in the gradient, LR and WEIGHT_DECAY of the TRAIN section)
+        over all parameters, as insmos_amd.optim.AdamW; options override its arguments (decoupled=True, state_bits=8, max_grad_norm=...)."""
+        from .optim import AdamW
+        tc = self.cfg["TRAIN"]
+        options = {"lr": float(tc["LR"]), "weight_decay": float(tc.get("WEIGHT_DECAY", 0.0)), "decoupled": False, **options}
+        return AdamW(list(self.params.values()), **options)
+
     def sgd_step(self, lr):
         with torch.no_grad():
             for v in self.params.values():

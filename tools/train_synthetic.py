@@ -5,7 +5,8 @@
     python tools/train_synthetic.py --steps 20 [--n-az 472] [--out /tmp/insmos_synth.ckpt]
     python -m torch.distributed.run --nproc-per-node 8 --master-addr 127.0.0.1 tools/train_synthetic.py --steps 20
 
-Optimiser and schedule as models/models.py:188-193 (Adam(lr, weight_decay) + StepLR(step_size=LR_EPOCH, gamma=LR_DECAY));
+Optimiser and schedule as models/models.py:188-193 (Adam(lr, weight_decay) + StepLR(step_size=LR_EPOCH, gamma=LR_DECAY)); --optimizer hip runs
+that Adam as one short chain of launches over all parameters (insmos_amd.optim.AdamW), hip8 with its moments in 8 bits;
 gradients are exchanged with insmos_amd.ddp.BucketedGradReducer (one RCCL all-reduce per 8 MB bucket) when WORLD_SIZE > 1.
 The trained tensors go back into a Lightning-shaped checkpoint that insmos_amd.models.InsMOSNet / predict_mos load.
 (Written at the end of round 1 after the GPU budget was spent: the pieces it calls are tested, this loop itself has not run.)"""
@@ -44,6 +45,8 @@ def main():
     ap.add_argument("--steps-per-epoch", type=int, default=5, help="the LR schedule steps once per this many iterations")
     ap.add_argument("--n-az", type=int, default=472)
     ap.add_argument("--out", type=str, default=None)
+    ap.add_argument("--optimizer", choices=("torch", "hip", "hip8"), default="torch")
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="clip by the global norm (hip, hip8)")
     args = ap.parse_args()
     rank, world, local = (int(os.environ.get(k, d)) for k, d in (("RANK", 0), ("WORLD_SIZE", 1), ("LOCAL_RANK", 0)))
     torch.cuda.set_device(local)
@@ -54,7 +57,10 @@ def main():
     cfg = P.default_cfg()
     sd = P.random_state_dict(cfg, 0, cls_bias=-2.0, box_w_std=0.05)
     tr = InsMOSTrainer(cfg, sd, dev)
-    opt = torch.optim.Adam(list(tr.params.values()), lr=float(cfg["TRAIN"]["LR"]), weight_decay=float(cfg["TRAIN"]["WEIGHT_DECAY"]))
+    if args.optimizer == "torch":
+        opt = torch.optim.Adam(list(tr.params.values()), lr=float(cfg["TRAIN"]["LR"]), weight_decay=float(cfg["TRAIN"]["WEIGHT_DECAY"]))
+    else:
+        opt = tr.make_optimizer(state_bits=8 if args.optimizer == "hip8" else 32, max_grad_norm=args.max_grad_norm)
     sched = torch.optim.lr_scheduler.StepLR(opt, step_size=int(cfg["TRAIN"]["LR_EPOCH"]), gamma=float(cfg["TRAIN"]["LR_DECAY"]))
     reducer = tr.make_reducer() if world > 1 else None
     for step in range(args.steps):
