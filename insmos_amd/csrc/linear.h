@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(256) k_linear_join(const GemmP p) {
 // columns and all of k, its 8 waves take 128 bytes of k in turn and add up in LDS.  Fragments come straight from memory (KC) or, for weights
 // with contiguous columns, through a turn of 16 x 32 values in the wave's own LDS; the whole of a wave's weights is in flight at once.
 // Rows and columns behind the matrix repeat the last one and are not stored; k behind its end is zero in both operands.
-// 1 x 2048 x 8192 bf16: %s against %s us with the flat tiles and a join.
+// 1 x 2048 x 8192 bf16: 7.0 us (4.8 TB/s of weights) against 6.0 + 4.2 with the flat tiles and a join.
 // eight values from k on, zeros behind K, one by one
 template <class T>
 __device__ __forceinline__ s16x8 load_k8(const T* row, int k, int K) {

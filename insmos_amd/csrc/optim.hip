@@ -6,7 +6,7 @@
 //   p  = p (1 - lr wd or 1) - lr / (1 - b1^t) * (m / (sqrt(v) / sqrt(1 - b2^t) + eps))
 //
 // Bound: HBM.  An element moves 28 bytes with fp32 tensors and moments (p, m, v read and written, g read; + 4 when the norm is
-// taken), 16 with moments in 8 bits; the arithmetic is some 20 (32 bits) or 80 (8 bits) vector instructions per element.
+// taken), 16 with moments in 8 bits; the arithmetic is some 45 (32 bits) or 75 (8 bits) vector instructions per element.
 //
 // Layout: the moments (and fp32 master weights) of a list lie in ONE buffer each; tensor i starts at a multiple of 256 elements, so
 // their accesses are 16-byte ones whatever the tensors are, and only p and g come with an address each.  The addresses travel as
@@ -28,7 +28,7 @@ namespace {
 
 constexpr int OPT_BLOCK = 256;      // elements per scale and alignment of a tensor in the state buffers
 constexpr int STEP_CHUNK = 4096;    // elements per workgroup of the step: 4 x (4 per lane x 256 lanes)
-constexpr int NORM_CHUNK = 8192;    // ... of the norm (one 8-byte partial sum each)
+constexpr int NORM_CHUNK = 8192;    // ... of the norm (one 8-byte partial sum each); 16 bytes a lane and load
 constexpr int64_t PART = 1 << 30;   // a longer tensor travels as several entries of this many elements
 
 // A launch's arguments may have 4 KB: 140 entries of 28 bytes for the step, 250 of 16 for the norm.
@@ -59,12 +59,8 @@ struct StepVals {   // what the launches of one step share (device memory)
 };
 
 typedef float of32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 obf16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 of16x4 __attribute__((ext_vector_type(4)));
-template <class T> struct Vec4;
-template <> struct Vec4<float> { typedef of32x4 t; };
-template <> struct Vec4<__bf16> { typedef obf16x4 t; };
-template <> struct Vec4<_Float16> { typedef of16x4 t; };
+typedef float of32x8 __attribute__((ext_vector_type(8)));
+template <class T, int V> struct VecOf { typedef T t __attribute__((ext_vector_type(V))); };
 
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {
     x ^= x >> 16; x *= 0x7FEB352Du;
@@ -81,54 +77,62 @@ __device__ __forceinline__ int tensor_of(const List& L, uint32_t b) {
     }
     return lo;
 }
-// four elements of a tensor from element i on; zeros past its end; `wide` = the tensor's address allows one access
-template <class T>
-__device__ __forceinline__ of32x4 load4(const T* __restrict__ p, uint32_t i, uint32_t n, bool wide) {
-    if (wide && i + 4 <= n) return __builtin_convertvector(*(const typename Vec4<T>::t*)(p + i), of32x4);
-    of32x4 r = {0.f, 0.f, 0.f, 0.f};
+// V (4 or 8) elements of a tensor from element i on; zeros past its end; `wide` = the tensor's address allows one access
+template <int V, class T>
+__device__ __forceinline__ typename VecOf<float, V>::t load_v(const T* __restrict__ p, uint32_t i, uint32_t n, bool wide) {
+    typedef typename VecOf<float, V>::t FV;
+    if (wide && i + V <= n) return __builtin_convertvector(*(const typename VecOf<T, V>::t*)(p + i), FV);
+    FV r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (i + j < n) r[j] = (float)p[i + j];
+    for (int j = 0; j < V; ++j) r[j] = i + j < n ? (float)p[i + j] : 0.f;
     return r;
 }
-template <class T>
-__device__ __forceinline__ void store4(T* __restrict__ p, uint32_t i, uint32_t n, bool wide, of32x4 v) {
-    if (wide && i + 4 <= n) { *(typename Vec4<T>::t*)(p + i) = __builtin_convertvector(v, typename Vec4<T>::t); return; }
+template <int V, class T>
+__device__ __forceinline__ void store_v(T* __restrict__ p, uint32_t i, uint32_t n, bool wide, typename VecOf<float, V>::t v) {
+    typedef typename VecOf<T, V>::t TV;
+    if (wide && i + V <= n) { *(TV*)(p + i) = __builtin_convertvector(v, TV); return; }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < V; ++j)
         if (i + j < n) p[i + j] = (T)v[j];
 }
-template <class T>
-__device__ __forceinline__ bool is_wide(const void* a) { return ((uintptr_t)a & (4 * sizeof(T) - 1)) == 0; }
+// (a vector of 32 bytes is two accesses of 16)
+template <class T, int V>
+__device__ __forceinline__ bool is_wide(const void* a) { return ((uintptr_t)a & (V * sizeof(T) < 16 ? V * sizeof(T) - 1 : 15)) == 0; }
 
 // ---- the gradients' sum of squares: one fp64 partial per workgroup (fixed order: the same bits every time) ------------------
 // Four squares are added in fp32 (their rounding errors have no direction and average out) and the sums in fp64: a quarter of the
 // fp64 work.  Sums near fp32's limits are taken in fp64.
-__device__ __forceinline__ void add_squares(double& s, const of32x4 v) {
-    const float q = fmaf(v[0], v[0], v[1] * v[1]) + fmaf(v[2], v[2], v[3] * v[3]);
-    if (q >= 1e-30f && q <= 1e37f) s += (double)q;
-    else
+template <int V>
+__device__ __forceinline__ void add_squares(double& s, const typename VecOf<float, V>::t v) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s = fma((double)v[j], (double)v[j], s);
+    for (int h = 0; h < V; h += 4) {
+        const float q = fmaf(v[h], v[h], v[h + 1] * v[h + 1]) + fmaf(v[h + 2], v[h + 2], v[h + 3] * v[h + 3]);
+        if (q >= 1e-30f && q <= 1e37f) s += (double)q;
+        else
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s = fma((double)v[h + j], (double)v[h + j], s);
+    }
 }
 template <class T>
 __global__ void __launch_bounds__(256) k_grad_sumsq(const NormList L, double* __restrict__ partial) {
+    constexpr int V = 16 / sizeof(T), STEP = 256 * V;
+    typedef typename VecOf<float, V>::t FV;
+    typedef typename VecOf<T, V>::t TV;
     const int t = tensor_of(L, blockIdx.x);
     const T* g = (const T*)L.g[t];
     const uint32_t n = L.n[t], base = (blockIdx.x - L.first[t]) * NORM_CHUNK;
-    const bool wide = is_wide<T>(g);
+    const bool wide = is_wide<T, V>(g);
     double s = 0.0;
     if (wide && base + NORM_CHUNK <= n) {   // a whole chunk: all loads in flight
-        of32x4 v[NORM_CHUNK / 1024];
+        TV v[NORM_CHUNK / STEP];
 #pragma unroll
-        for (int u = 0; u < NORM_CHUNK / 1024; ++u)
-            v[u] = __builtin_convertvector(*(const typename Vec4<T>::t*)(g + base + u * 1024 + threadIdx.x * 4), of32x4);
+        for (int u = 0; u < NORM_CHUNK / STEP; ++u) v[u] = *(const TV*)(g + base + u * STEP + threadIdx.x * V);
 #pragma unroll
-        for (int u = 0; u < NORM_CHUNK / 1024; ++u) add_squares(s, v[u]);
+        for (int u = 0; u < NORM_CHUNK / STEP; ++u) add_squares<V>(s, __builtin_convertvector(v[u], FV));
     } else {
-        for (int u = 0; u < NORM_CHUNK / 1024; ++u) {
-            const uint32_t i = base + u * 1024 + threadIdx.x * 4;
-            if (i < n) add_squares(s, load4(g, i, n, wide));
+        for (int u = 0; u < NORM_CHUNK / STEP; ++u) {
+            const uint32_t i = base + u * STEP + threadIdx.x * V;
+            if (i < n) add_squares<V>(s, load_v<V>(g, i, n, wide));
         }
     }
 #pragma unroll
@@ -171,12 +175,14 @@ __global__ void __launch_bounds__(1024) k_adamw_prepare(const PrepareP A) {
     __shared__ double w[16];
     double norm = 0.0;
     if (A.partial) norm = sqrt(sum_partials(A.partial, A.n_partial, w));
-    if (threadIdx.x) return;
+    if (threadIdx.x > 1) return;
     if (A.norm_in) norm = (double)*A.norm_in;
-    if (A.norm_out) *A.norm_out = (float)norm;
     StepVals v;
     v.skip = A.skip_nonfinite && !(norm <= 1.7976931348623157e308);
     const int t = *A.step + (v.skip ? 0 : 1);
+    const double power = pow(threadIdx.x ? A.b2 : A.b1, (double)t), power2 = __shfl(power, 1);   // lane 0: b1^t, lane 1: b2^t
+    if (threadIdx.x) return;
+    if (A.norm_out) *A.norm_out = (float)norm;
     *A.step = t;
     const double lr = A.lr_dev ? (double)*A.lr_dev : A.lr;
     v.clip = 1.f;
@@ -185,8 +191,8 @@ __global__ void __launch_bounds__(1024) k_adamw_prepare(const PrepareP A) {
         v.clip = c >= 1.f ? 1.f : c;   // (a norm that is NaN stays one)
     }
     v.keep = A.decoupled ? (float)(1.0 - lr * A.wd) : 1.f;
-    v.size = (float)(lr / (1.0 - pow(A.b1, (double)t)));
-    v.root = (float)(1.0 / sqrt(1.0 - pow(A.b2, (double)t)));
+    v.size = (float)(lr / (1.0 - power));
+    v.root = (float)(1.0 / sqrt(1.0 - power2));
     v.key = mix32(mix32((uint32_t)t) ^ A.seed);
     *A.vals = v;
 }
@@ -208,24 +214,34 @@ __device__ __forceinline__ uint32_t code_of(float a, float inv, uint32_t u16) {
     const float y = fminf(a * inv, 448.f) * 0x1p-120f;
     return (__float_as_uint(y) + (u16 << 4)) >> 20;
 }
-// the largest of the wave's 64 values in a scalar register (row shifts, then the rows' last lanes handed on)
-__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false));   // row_shr:1, 2, 4, 8
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false));
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false));
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false));
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));   // row_bcast:15, 31
-    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));
-    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+// the largest value of each half of the wave, in all of its lanes: rotations within the rows of 16, then the rows of a half exchanged
+__device__ __forceinline__ uint32_t half_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));   // row_ror:8, 4, 2, 1
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false));
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return max((uint32_t)r[0], (uint32_t)r[1]);
 }
-__device__ __forceinline__ of32x4 decode4(uint32_t c, float scale) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
-    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-    of32x4 r = {lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
+__device__ __forceinline__ of32x8 decode8(uint2 c, float scale) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x, true);
+    const auto d = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.y, true);
+    of32x8 r = {a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale, d[0] * scale, d[1] * scale, e[0] * scale, e[1] * scale};
     return r;
 }
+// Root and quotient with one correction of v_rsq's / v_rcp's result: the correctly rounded value but for about one argument in a million (one
+// unit in the last place off there), at half of the general functions' instructions.  x in 2^-96 .. 2^96; d = a root of that times a factor + eps.
+__device__ __forceinline__ float root_of(float x) {
+    const float y = __builtin_amdgcn_rsqf(x), s = x * y;
+    return fmaf(fmaf(-s, s, x), 0.5f * y, s);
+}
+__device__ __forceinline__ float quotient(float a, float d) {
+    const float y = __builtin_amdgcn_rcpf(d), q = a * y;
+    return fmaf(fmaf(-d, q, a), y, q);
+}
 
-template <class T, int BITS, bool MASTER>
+// Moments in 32 bits: 4 elements a lane.
+template <class T, bool MASTER>
 __global__ void __launch_bounds__(256) k_adamw(const StepList L, const StepP A) {
     const StepVals S = *A.vals;
     if (S.skip) return;
@@ -233,92 +249,130 @@ __global__ void __launch_bounds__(256) k_adamw(const StepList L, const StepP A) 
     T* p = (T*)L.p[t];
     const T* g = (const T*)L.g[t];
     const uint32_t n = L.n[t], base = (blockIdx.x - L.first[t]) * STEP_CHUNK;
-    const uint32_t lane4 = (threadIdx.x & 63) * 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const bool wide = is_wide<T>(p) && is_wide<T>(g);
+    const bool wide = is_wide<T, 4>(p) && is_wide<T, 4>(g);
+    const int64_t off = (int64_t)L.off[t] * OPT_BLOCK;
 #pragma unroll
     for (int u = 0; u < STEP_CHUNK / 1024; ++u) {
-        const uint32_t from = base + u * 1024 + wave * 256, i = from + lane4;   // a wave's 256 elements are one block of the state
-        if (from >= n) break;
-        const int64_t b = (int64_t)L.off[t] + from / OPT_BLOCK, s = b * OPT_BLOCK + lane4;
-        of32x4 gr = load4(g, i, n, wide);
-        of32x4 pr = MASTER ? *(const of32x4*)(A.masters + s) : load4((const T*)p, i, n, wide);
-        of32x4 m, v;
-        if (BITS == 32) {
-            m = *(const of32x4*)((const float*)A.m + s);
-            v = *(const of32x4*)((const float*)A.v + s);
-        } else {
-            m = decode4(*(const uint32_t*)((const uint8_t*)A.m + s), A.scales[b]);
-            v = decode4(*(const uint32_t*)((const uint8_t*)A.v + s), A.scales[A.n_blocks + b]);
-            v = v * v;
-        }
-        of32x4 root, np;
+        const uint32_t i = base + u * 1024 + threadIdx.x * 4;
+        if ((i & ~(uint32_t)(OPT_BLOCK - 1)) >= n) break;   // (a wave's 256 elements are one block of the state)
+        const int64_t s = off + i;
+        const of32x4 gr = load_v<4>(g, i, n, wide), pr = MASTER ? *(const of32x4*)(A.masters + s) : load_v<4>((const T*)p, i, n, wide);
+        of32x4 m = *(const of32x4*)((const float*)A.m + s), v = *(const of32x4*)((const float*)A.v + s), np;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float gj = gr[j] * S.clip;
             if (A.coupled) gj = gj + A.wd * pr[j];
             m[j] = A.b1 * m[j] + A.a1 * gj;
             v[j] = A.b2 * v[j] + A.a2 * (gj * gj);
-            root[j] = sqrtf(v[j]);
-            np[j] = pr[j] * S.keep - S.size * (m[j] / (root[j] * S.root + A.eps));
+            np[j] = pr[j] * S.keep - S.size * (m[j] / (sqrtf(v[j]) * S.root + A.eps));
+            if (i + j >= n) m[j] = v[j] = np[j] = 0.f;   // behind the tensor's end the state holds zeros
+        }
+        if (MASTER) *(of32x4*)(A.masters + s) = np;
+        store_v<4>(p, i, n, wide, np);
+        *(of32x4*)((float*)A.m + s) = m;
+        *(of32x4*)((float*)A.v + s) = v;
+    }
+}
+
+// Moments in 8 bits: 8 elements a lane, a block is half a wave.  Bound by the vector instructions (some 75 per element, the hash's two products
+// and the codes among them) as much as by its bytes: 200 M bf16 parameters 395 us, their 2 GB at 5.5 TB/s 364; with 4 elements a lane, the general
+// root and division and the wave's maximum through the LDS 546.
+template <class T, bool MASTER>
+__global__ void __launch_bounds__(256) k_adamw8(const StepList L, const StepP A) {
+    const StepVals S = *A.vals;
+    if (S.skip) return;
+    const int t = tensor_of(L, blockIdx.x);
+    T* p = (T*)L.p[t];
+    const T* g = (const T*)L.g[t];
+    const uint32_t n = L.n[t], base = (blockIdx.x - L.first[t]) * STEP_CHUNK;
+    const bool wide = is_wide<T, 8>(p) && is_wide<T, 8>(g);
+    constexpr uint32_t INF = 0x7F800000u;
+#pragma unroll
+    for (int u = 0; u < STEP_CHUNK / 2048; ++u) {
+        const uint32_t i = base + u * 2048 + threadIdx.x * 8, from = i & ~(uint32_t)(OPT_BLOCK - 1);
+        if (from >= n) break;   // (the same for the half wave: what follows exchanges values within halves)
+        const int64_t b = (int64_t)L.off[t] + from / OPT_BLOCK, s = b * OPT_BLOCK + (i - from);
+        const of32x8 gr = load_v<8>(g, i, n, wide), pr = MASTER ? *(const of32x8*)(A.masters + s) : load_v<8>((const T*)p, i, n, wide);
+        of32x8 m = decode8(*(const uint2*)((const uint8_t*)A.m + s), A.scales[b]);
+        of32x8 v = decode8(*(const uint2*)((const uint8_t*)A.v + s), A.scales[A.n_blocks + b]);
+        of32x8 root, np;
+        float least = 1.f, most = 1.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float gj = gr[j] * S.clip;
+            if (A.coupled) gj = gj + A.wd * pr[j];
+            m[j] = A.b1 * m[j] + A.a1 * gj;
+            v[j] = A.b2 * (v[j] * v[j]) + A.a2 * (gj * gj);
+            least = fminf(least, v[j]);
+            most = fmaxf(most, v[j]);
+            if (!(v[j] == v[j])) most = 3e38f;
+        }
+        if (least >= 0x1p-96f && most <= 0x1p96f) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                root[j] = root_of(v[j]);
+                np[j] = pr[j] * S.keep - S.size * quotient(m[j], root[j] * S.root + A.eps);
+            }
+        } else {   // zeros (no gradient ever), far values
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                root[j] = sqrtf(v[j]);
+                np[j] = pr[j] * S.keep - S.size * (m[j] / (root[j] * S.root + A.eps));
+            }
         }
         if (from + OPT_BLOCK > n) {   // behind the tensor's end the state holds zeros
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (i + j >= n) m[j] = v[j] = root[j] = np[j] = 0.f;
+            for (int j = 0; j < 8; ++j)
+                if (i + j >= n) m[j] = root[j] = np[j] = 0.f;
         }
-        if (MASTER) *(of32x4*)(A.masters + s) = np;
-        store4(p, i, n, wide, np);
-        if (BITS == 32) {
-            *(of32x4*)((float*)A.m + s) = m;
-            *(of32x4*)((float*)A.v + s) = v;
-        } else {
-            // Largest magnitudes as integers (the same order as the floats'; inf and NaN are above all finite ones).  sqrt(v) has no
-            // sign but that of a NaN.
-            uint32_t am[4], ar[4], hm = 0, hs = 0;
+        if (MASTER) *(of32x8*)(A.masters + s) = np;
+        store_v<8>(p, i, n, wide, np);
+        // Largest magnitudes as integers (the same order as the floats'; inf and NaN are above all finite ones).  sqrt(v) has no sign but that
+        // of a NaN.
+        uint32_t am[8], ar[8], hm = 0, hs = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                am[j] = __float_as_uint(m[j]) & 0x7FFFFFFFu;
-                ar[j] = __float_as_uint(root[j]) & 0x7FFFFFFFu;
-                hm = max(hm, am[j]);
-                hs = max(hs, ar[j]);
+        for (int j = 0; j < 8; ++j) {
+            am[j] = __float_as_uint(m[j]) & 0x7FFFFFFFu;
+            ar[j] = __float_as_uint(root[j]) & 0x7FFFFFFFu;
+            hm = max(hm, am[j]);
+            hs = max(hs, ar[j]);
+        }
+        uint32_t tm = half_max(hm), ts = half_max(hs);
+        const bool fine = max(tm, ts) < INF;   // (the same for the half wave)
+        if (!fine) {
+            hm = hs = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                hm = max(hm, am[j] < INF ? am[j] : 0u);
+                hs = max(hs, ar[j] < INF ? ar[j] : 0u);
             }
-            uint32_t tm = wave_max(hm), ts = wave_max(hs);
-            const bool fine = max(tm, ts) < 0x7F800000u;   // (the same for the wave)
+            tm = half_max(hm);
+            ts = half_max(hs);
+        }
+        const float km = fmaxf(__uint_as_float(tm) * (1.f / 448.f), 0x1p-126f), ks = fmaxf(__uint_as_float(ts) * (1.f / 448.f), 0x1p-126f);
+        const int inv = (int)__float_as_uint(1.f / ((threadIdx.x & 1) ? ks : km));   // both divisions at once, in the odd and the even lanes
+        const float im = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, inv, 0xA0, 0xf, 0xf, false));   // quad_perm:[0,0,2,2]
+        const float is = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, inv, 0xF5, 0xf, 0xf, false));   // quad_perm:[1,1,3,3]
+        const uint32_t at = (uint32_t)s + (uint32_t)((uint64_t)s >> 32) * 0x9E3779B1u + S.key;   // (8 | s: no carry in s + j)
+        uint32_t cm[2] = {0, 0}, cs[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t h = mix32(at + j);
+            uint32_t a = code_of(__uint_as_float(am[j]), im, h & 0xFFFFu), r = code_of(__uint_as_float(ar[j]), is, h >> 16);
+            r = max(r, min(ar[j], 1u));
             if (!fine) {
-                hm = hs = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    hm = max(hm, am[j] < 0x7F800000u ? am[j] : 0u);
-                    hs = max(hs, ar[j] < 0x7F800000u ? ar[j] : 0u);
-                }
-                tm = wave_max(hm);
-                ts = wave_max(hs);
+                if (am[j] >= INF) a = 0x7Fu;
+                if (ar[j] >= INF) r = 0x7Fu;
             }
-            const float km = fmaxf(__uint_as_float(tm) * (1.f / 448.f), 0x1p-126f), ks = fmaxf(__uint_as_float(ts) * (1.f / 448.f), 0x1p-126f);
-            const float inv = 1.f / ((threadIdx.x & 1) ? ks : km);   // both divisions at once, in the odd and the even lanes
-            const float im = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(inv), 0));
-            const float is = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(inv), 1));
-            const uint32_t at = (uint32_t)s + (uint32_t)((uint64_t)s >> 32) * 0x9E3779B1u + S.key;   // (256 | s: no carry in s + j)
-            uint32_t cm = 0, cs = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t h = mix32(at + j);
-                uint32_t a = code_of(__uint_as_float(am[j]), im, h & 0xFFFFu), r = code_of(__uint_as_float(ar[j]), is, h >> 16);
-                r = max(r, min(ar[j], 1u));
-                if (!fine) {
-                    if (am[j] >= 0x7F800000u) a = 0x7Fu;
-                    if (ar[j] >= 0x7F800000u) r = 0x7Fu;
-                }
-                a |= (__float_as_uint(m[j]) >> 24) & 0x80u;
-                cm |= a << (8 * j);
-                cs |= r << (8 * j);
-            }
-            *(uint32_t*)((uint8_t*)A.m + s) = cm;
-            *(uint32_t*)((uint8_t*)A.v + s) = cs;
-            if (lane4 == 0) {
-                A.scales[b] = km;
-                A.scales[A.n_blocks + b] = ks;
-            }
+            a |= (__float_as_uint(m[j]) >> 24) & 0x80u;
+            cm[j / 4] |= a << (8 * (j % 4));
+            cs[j / 4] |= r << (8 * (j % 4));
+        }
+        *(uint2*)((uint8_t*)A.m + s) = make_uint2(cm[0], cm[1]);
+        *(uint2*)((uint8_t*)A.v + s) = make_uint2(cs[0], cs[1]);
+        if (i == from) {
+            A.scales[b] = km;
+            A.scales[A.n_blocks + b] = ks;
         }
     }
 }
@@ -381,17 +435,16 @@ int sumsq(const InsmosOptTensor* tensors, int n, int dtype, double* partial, hip
     *used = at;
     return rc;
 }
-template <class T, int BITS, bool MASTER>
-int launch_step(const StepList& L, uint32_t blocks, const StepP& P, hipStream_t s) {
-    const auto kernel = k_adamw<T, BITS, MASTER>;
+template <class T, bool MASTER>
+int launch_step(const StepList& L, uint32_t blocks, const StepP& P, int bits, hipStream_t s) {
+    const auto kernel = bits == 32 ? k_adamw<T, MASTER> : k_adamw8<T, MASTER>;
     INSMOS_LAUNCH(kernel, dim3(blocks), dim3(256), 0, s, L, P);
     HIP_TRY(hipGetLastError());
     return INSMOS_OK;
 }
 template <class T>
 int launch_step_t(const StepList& L, uint32_t blocks, const StepP& P, int bits, hipStream_t s) {
-    if (P.masters) return bits == 32 ? launch_step<T, 32, true>(L, blocks, P, s) : launch_step<T, 8, true>(L, blocks, P, s);
-    return bits == 32 ? launch_step<T, 32, false>(L, blocks, P, s) : launch_step<T, 8, false>(L, blocks, P, s);
+    return P.masters ? launch_step<T, true>(L, blocks, P, bits, s) : launch_step<T, false>(L, blocks, P, bits, s);
 }
 bool good_list(const InsmosOptTensor* t, int n, int dtype) {
     return (t || !n) && n >= 0 && (dtype == INSMOS_F32 || dtype == INSMOS_BF16 || dtype == INSMOS_F16);
@@ -474,8 +527,7 @@ extern "C" int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tens
     P.wd = (float)weight_decay;
     P.coupled = !decoupled && weight_decay != 0.0;
     return each_launch<StepList>(tensors_host, n_tensors, STEP_CHUNK, true, dtype, n_state, [&](const StepList& L, uint32_t blocks) -> int {
-        if (dtype == INSMOS_F32)
-            return state_bits == 32 ? launch_step<float, 32, false>(L, blocks, P, s) : launch_step<float, 8, false>(L, blocks, P, s);
+        if (dtype == INSMOS_F32) return launch_step<float, false>(L, blocks, P, state_bits, s);
         return dtype == INSMOS_BF16 ? launch_step_t<__bf16>(L, blocks, P, state_bits, s) : launch_step_t<_Float16>(L, blocks, P, state_bits, s);
     });
 }
