@@ -852,8 +852,8 @@ int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dt
  *   z = x W + bias (+ residual if residual_first);   y = act(z) (+ residual if !residual_first)
  * x (M, K), row pitch ld_x; W (K, N) with row pitch ld_w, or given as (N, K) rows with w_out_in; bias (N) or NULL; residual (M, N), any row
  * pitch >= 0 (0: one row for all), or NULL; y (M, N).  All of one dtype (INSMOS_F32 / BF16 / F16), pitches in elements (at most 2^20, as are
- * K and N); sums in fp32, one rounding per output.  Addresses and pitches need only the elements' alignment; operands that are not 16-byte
- * aligned are laid out again in ws.  slope: NULL, or receives act'(z) for the backward pass, in fp32 for INSMOS_F32 and otherwise as 16 bits
+ * K and N); sums in fp32, one rounding per output.  Addresses and pitches need only the elements' alignment; 16-bit operands at odd
+ * addresses or pitches are laid out again in ws.  slope: NULL, or receives act'(z) for the backward pass, in fp32 for INSMOS_F32 and otherwise as 16 bits
  * (steps of 2^-15 from -1/2; 0xFFFF: not a number), 16-byte aligned, ld_slope a multiple of 16 bytes that holds N rounded up to 16 bytes; not
  * without an activation.
  * Backward: dz = dy act'(z);  dx = dz W^T;  dw = x^T dz in the weight's layout;  db = column sums of dz (before its rounding to the type).

@@ -7,8 +7,8 @@
 // a transposed (cout, cin) weight, dz W^T the other way round, x^T dz is (NC, NC).  Nothing is transposed in memory.
 //
 // A tile row of either operand is 128 bytes of LDS (64 16-bit or 32 fp32 values of k for KC, or BK rows of R values for NC); a wave
-// instruction moves 64 x 16 bytes from memory straight to LDS (buffer_load ... lds), with the buffer's extent as the bounds check:
-// rows behind the matrix read as zero, and so does k behind its end.  Two tiles in LDS: one is filled while the other is read.
+// instruction moves 64 x 16 bytes from memory straight to LDS (buffer_load ... lds; addresses on 4 bytes), with the buffer's extent as the
+// bounds check: rows behind the matrix read as zero, and so does k behind its end (cut() clears a chunk that K ends in).  Two tiles in LDS: one is filled while the other is read.
 // The LDS image is written in lane order, so the bank swizzle is in the ADDRESSES READ: 16-byte chunk c of KC row r lies at c ^ (r & 7)
 // (the 8 lanes of a read phase then touch 8 different chunks), chunk c of NC row k at c ^ 4 (k & 3 | k >> 1 & 4) (the 8 rows of a
 // transposing read touch 8 different 64-byte pieces).  NC operands reach the matrix instructions through ds_read_b64_tr_b16.
@@ -176,9 +176,10 @@ struct Tile {
 
     static __device__ __forceinline__ int swizzle(int k) { return ES == 2 ? ((((k & 3) | ((k >> 1) & 4)) << 2)) & (CPR - 1) : 0; }
     __device__ __forceinline__ void init(const void* base, int64_t ld, int r0, int rtot, int K, int kt0, int wave, int lane) {
+        // (the bounds check goes by dwords: the one that holds the operand's last value counts as inside)
         if (LAY == KC) {
             p = (const char*)base + (int64_t)r0 * ld * ES;
-            left = ((int64_t)(min(R, rtot - r0) - 1) * ld + (K + CE - 1) / CE * CE) * ES;   // (rows are whole chunks, see loadable())
+            left = (((int64_t)(min(R, rtot - r0) - 1) * ld + K) * ES + 3) & ~(int64_t)3;
             step = 128;
             chunk = ((lane & 7) ^ (lane >> 3)) * CE;
             voff = (uint32_t)((wave * 8 + (lane >> 3)) * ld * ES) + chunk * ES;
@@ -186,7 +187,6 @@ struct Tile {
         } else {
             static_assert(NI == 1 || ES == 4 || NW * RPI % 16 == 0, "one swizzle for a lane's instructions");
             p = (const char*)base + (int64_t)r0 * ES;
-            // (the check goes by dwords: the one that holds the last value counts as inside)
             left = (((int64_t)(K - 1) * ld + (rtot - r0)) * ES + 3) & ~(int64_t)3;
             step = (int64_t)BK * ld * ES;
             const int k = wave * RPI + lane / CPR;
@@ -206,6 +206,17 @@ struct Tile {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LIN_LDS void*)(lds + (i * NW + wave) * 1024), 16, v, i * istep, 0, 0);
         p += step;
         left -= step;
+    }
+    // KC: the chunk that K ends in has brought values from behind the row's end; zeros in their place (k: valid values of the tile)
+    static __device__ __forceinline__ void cut(LIN_LDS char* lds, int k) {
+        if (LAY != KC || k % CE == 0) return;
+        for (int r = threadIdx.x; r < R; r += NW * 64) {
+            LIN_LDS char* c = lds + r * 128 + (((k / CE) ^ (r & 7)) << 4);
+            for (int e = k % CE; e < CE; ++e) {
+                if (ES == 2) *(LIN_LDS short*)(c + e * 2) = 0;
+                else *(LIN_LDS float*)(c + e * 4) = 0.f;
+            }
+        }
     }
 };
 
@@ -446,6 +457,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_gemm(const GemmP p) 
         __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): the first tile has arrived
         __syncthreads();
         for (int kt = it.kt0; kt < it.kt1; ++kt) {
+            if ((LA == KC || LB == KC) && kt == nk - 1 && p.K % (16 / (int)sizeof(T))) {
+                G::TA::cut(L + cur, p.K - kt * BK);
+                G::TB::cut(L + cur + SA, p.K - kt * BK);
+                __syncthreads();
+            }
             G::step(L + (cur ^ (SA + SB)), L + cur, ta, tb, fa, fb, regs, acc, kt + 1 < it.kt1, p.K - (kt + 1) * BK, wave);
             cur ^= SA + SB;
             __builtin_amdgcn_s_waitcnt(0x0F70);   // the next tile has arrived, for every wave, and all are done with this one

@@ -13,22 +13,24 @@ namespace {
 size_t size_of(int dtype) { return dtype == INSMOS_F32 ? 4 : 2; }
 
 // ---- operands that need another layout --------------------------------------------------------------------------------------
-// The tile loads move 16 aligned bytes: address and row pitch must be multiples of 16 bytes, and where k is the contiguous index it must be a
-// multiple of a chunk (a chunk half behind k would bring the next row's values in).  Other operands are copied into rows padded with zeros;
-// the copy's time is that of its bytes, the product's an order more.
-template <class T>
-__global__ void __launch_bounds__(256) k_linear_pack(const T* __restrict__ src, int64_t ld, int64_t rows, int cols, T* __restrict__ dst, int ld_dst) {
+// The tile loads move 16 bytes from any address on 4 bytes; 16-bit operands at odd addresses or pitches are copied into rows padded with zeros.
+__global__ void __launch_bounds__(256) k_linear_pack(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int cols, uint16_t* __restrict__ dst,
+                                                     int ld_dst) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    constexpr int V = 16 / sizeof(T);
+    constexpr int V = 8;
     const int per = ld_dst / V;
     const int64_t r = i / per;
     const int c = (int)(i % per) * V;
     if (r >= rows) return;
-    typedef T TV __attribute__((ext_vector_type(16 / sizeof(T))));
-    TV v;
+    typedef uint16_t U8 __attribute__((ext_vector_type(8), aligned(2)));
+    U8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (c + V <= cols) v = *(const U8*)(src + r * ld + c);
+    else
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = c + e < cols ? src[r * ld + c + e] : (T)0;
-    *(TV*)(dst + r * ld_dst + c) = v;
+        for (int e = 0; e < V; ++e)
+            if (c + e < cols) v[e] = src[r * ld + c + e];
+    typedef uint16_t A8 __attribute__((ext_vector_type(8)));
+    *(A8*)(dst + r * ld_dst + c) = v;
 }
 struct Operand {
     const void* p;
@@ -36,25 +38,21 @@ struct Operand {
     int lay;
 };
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
-bool loadable(const void* p, int64_t ld, int contiguous, int lay, int dtype) {
-    const int64_t es = size_of(dtype), ce = 16 / es;
-    return (uintptr_t)p % 16 == 0 && ld % ce == 0 && (lay == NC || contiguous % ce == 0);
-}
+bool loadable(const void* p, int64_t ld, int dtype) { return (uintptr_t)p % 4 == 0 && ld * size_of(dtype) % 4 == 0; }
 size_t packed_bytes(int64_t rows, int cols, int dtype) {
     return pad256((size_t)rows * round_up(cols, 16 / (int)size_of(dtype)) * size_of(dtype));
 }
 // `rows` x `cols` (cols contiguous) as a loadable operand; copies into ws where it is none (any: the kernel takes it as it is)
 int operand(const void* p, int64_t ld, int64_t rows, int cols, int lay, int dtype, bool any, Bump& ws, hipStream_t s, Operand* out) {
     *out = {p, ld, lay};
-    if (any || loadable(p, ld, cols, lay, dtype)) return INSMOS_OK;
+    if (any || loadable(p, ld, dtype)) return INSMOS_OK;
     const int es = (int)size_of(dtype), to = round_up(cols, 16 / es);
     char* d = ws.take<char>((size_t)rows * to * es);
     if (!d) return INSMOS_EWORKSPACE;
     const int64_t threads = rows * (to / (16 / es));
     if ((threads + 255) / 256 > 0x7FFFFFFF / 256) return INSMOS_EINVAL;
     const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
-    if (dtype == INSMOS_F32) INSMOS_LAUNCH(k_linear_pack<uint32_t>, grid, block, 0, s, (const uint32_t*)p, ld, rows, cols, (uint32_t*)d, to);
-    else INSMOS_LAUNCH(k_linear_pack<uint16_t>, grid, block, 0, s, (const uint16_t*)p, ld, rows, cols, (uint16_t*)d, to);
+    INSMOS_LAUNCH(k_linear_pack, grid, block, 0, s, (const uint16_t*)p, ld, rows, cols, (uint16_t*)d, to);
     HIP_TRY(hipGetLastError());
     *out = {d, to, lay};
     return INSMOS_OK;
@@ -263,7 +261,7 @@ bool good_matrix(const void* p, int64_t ld, int64_t cols, int dtype) {
     return p && ld >= cols && ld <= (int64_t)1 << 20 && (uintptr_t)p % size_of(dtype) == 0;
 }
 // dz needs a buffer of its own where there is an activation or dy cannot be loaded as it is
-bool needs_dz(const void* dy, int64_t ld_dy, int N, int kind, int dtype) { return kind != INSMOS_SLOPE_NONE || !loadable(dy, ld_dy, N, KC, dtype); }
+bool needs_dz(const void* dy, int64_t ld_dy, int kind, int dtype) { return kind != INSMOS_SLOPE_NONE || !loadable(dy, ld_dy, dtype); }
 // rows of a buffer in the library's own layout: 16-byte aligned, whole chunks
 bool good_rows(const void* p, int64_t ld, int N, int dtype) {
     const int64_t chunk = 16 / (int64_t)size_of(dtype);
@@ -332,7 +330,7 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
     int rc = INSMOS_OK;
     const void* d = dy;
     int64_t ld_d = ld_dy;
-    const bool own = dz || ((dx || dw) && needs_dz(dy, ld_dy, N, slope_kind, dtype));
+    const bool own = dz || ((dx || dw) && needs_dz(dy, ld_dy, slope_kind, dtype));
     if (own || db) {
         SlopeP q = {};
         q.dy = dy; q.ld_dy = ld_dy;
@@ -360,9 +358,8 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
     }
     if (dx) {   // (M, K) = dz (M, N) W^T: k of this product is N
         Operand a, b;
-        const int np = round_up(N, (int)chunk);
         const bool any = plan_for((int)M, K, N, dtype, true).tile == FEW;
-        rc = operand(d, ld_d, M, own ? np : N, KC, dtype, any, bump, s, &a);   // (own rows end in zeros: N may count as padded there)
+        rc = operand(d, ld_d, M, N, KC, dtype, any, bump, s, &a);
         if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, NC, dtype, any, bump, s, &b) : operand(w, ld_w, K, N, KC, dtype, any, bump, s, &b);
         if (rc != INSMOS_OK) return rc;
         GemmP p = {};

@@ -111,7 +111,7 @@ def test_linear_against_float64(M, K, N, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("pads", [(8, 8, 8), (5, 3, 1), (1, 16, 2)])
-@pytest.mark.parametrize("M,K,N", [(7, 72, 40), (150, 40, 72), (260, 130, 134)])
+@pytest.mark.parametrize("M,K,N", [(7, 72, 40), (150, 40, 72), (260, 130, 134), (90, 33, 47), (140, 67, 129)])
 def test_linear_rows_of_any_pitch(M, K, N, pads, dtype):
     """Rows as slices of wider matrices with NaN between them: pitches that are and are not multiples of 16 bytes."""
     for layout in ("in_out", "out_in"):
@@ -356,8 +356,8 @@ def test_linear_entry_points_refuse():
                 {"slope": p}, {"slope": p + 4, "act": 2}, {"slope": p, "act": 2, "lds": 15}, {"ws": p + 8}, {"ldx": 1 << 21}):
         assert forward(**bad) == -1, bad
     assert forward(M=0) == 0
-    # a pitch that the tile loads cannot take, and no room for the copy
-    assert forward(M=200, ldx=9, n=0) == -3 and forward(M=200, ldx=9, ws=None) == -3
+    # 16-bit rows at an odd pitch, and no room for the copy
+    assert forward(M=200, ldx=9, dt=1, n=0) == -3 and forward(M=200, ldx=9, dt=2, ws=None) == -3
     assert lib.insmos_linear_ws_bytes(4, 0, 8, 0) == 0 and lib.insmos_linear_ws_bytes(4, 8, 8, 7) == 0
 
     def backward(dy=p, ldd=16, slope=None, lds=16, kind=0, x=p, ldx=8, w=p, ldw=16, M=4, K=8, N=16, dt=0, dx=p, lddx=8, dw=p, lddw=16, dz=None, lddz=16, ws=p, n=1024):
