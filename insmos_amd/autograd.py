@@ -492,7 +492,7 @@ _host_module = None
 
 
 def _host():
-    """The C++ side of linear(): argument checks, allocations and the library call (csrc/host_tensors.cpp)."""
+    """The C++ side of linear(): argument checks, allocations, the library calls and the autograd node (csrc/host_tensors.cpp)."""
     global _host_module
     if _host_module is None:
         lib = _lib.load()
@@ -501,30 +501,6 @@ def _host():
                                                                         lib.insmos_linear_backward, lib.insmos_linear_backward_ws_bytes)])
         _host_module = m
     return _host_module
-
-
-class LinearFunction(torch.autograd.Function):
-    """act(x W + b [+ r]) [+ r] with its gradients.  The backward keeps x, W and the activation's slopes (16 bits each with 16-bit types; y
-    itself for relu, whose slope is its sign)."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, residual_first):
-        # relu: y > 0 says what z > 0 does, unless a residual was added behind it
-        of_y = act == 1 and (residual is None or residual_first)
-        y, slope = _host().linear_forward(x, weight, bias, residual, act, residual_first, act != 0 and not of_y)
-        ctx.save_for_backward(x, weight, y if of_y else slope)
-        ctx.meta = (0 if act == 0 else 1 if of_y else 2, residual_first, bias is not None, residual is not None)   # INSMOS_SLOPE_*
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, slope = ctx.saved_tensors
-        kind, first, has_bias, has_res = ctx.meta
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        need_r = need_r and has_res
-        dx, dw, db, dz = _host().linear_backward(dy, slope, x, weight, kind, need_x, need_w, need_b and has_bias, need_r and first and kind != 0)
-        return dx, dw, db, (dz if dz is not None else dy) if need_r else None, None, None
 
 
 def linear(x, weight, bias=None, residual=None, activation=None, residual_first=False):
@@ -540,9 +516,7 @@ def linear(x, weight, bias=None, residual=None, activation=None, residual_first=
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"linear: activation is one of {list(_ACTIVATIONS)}, not {activation!r}") from None
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        return LinearFunction.apply(x, weight, bias, residual, act, bool(residual_first))
-    return _host().linear_forward(x, weight, bias, residual, act, residual_first, False)[0]
+    return _host().linear(x, weight, bias, residual, act, residual_first)
 
 
 # ---------------------------------------------------------------------------------------------------------------------

@@ -2,12 +2,15 @@
 // insmos_amd._host; nothing here runs on the GPU.
 //   opt_table: one pass over the optimiser step's lists that checks them and writes the InsmosOptTensor table (include/insmos_hip.h).  From
 //     Python the same pass costs ten attribute reads per tensor (some 0.1 us each: 0.5 ms for 250 tensors, ten times what the GPU needs).
-//   linear_forward / linear_backward: checks, allocations and the call of insmos_linear(_backward) (20 us from Python, where the GPU needs 7
-//     for one row).
+//   linear: the layer with its node on the autograd tape -- checks, allocations and the calls of insmos_linear(_backward) (20 us forward and
+//     90 with a backward from Python, where the GPU needs 7 for one row).
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -219,104 +222,153 @@ int64_t padded(int64_t cols, const at::Tensor& like) {
     return (cols + chunk - 1) / chunk * chunk;
 }
 
-// linear_forward(x, weight, bias or None, residual or None, act, residual_first, keep) -> (y, slopes for the backward pass or None)
-PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    return guarded([&]() -> PyObject* {
-        if (n_args != 7 || !g_linear) refuse("internal call");
-        const at::Tensor &x = arg(a[0], "x"), &w = arg(a[1], "weight");
-        const int act = (int)PyLong_AsLong(a[4]), first = PyObject_IsTrue(a[5]), keep = PyObject_IsTrue(a[6]);
-        const int dt = dtype_code(x.scalar_type());
-        std::string buf;
-        if (dt < 0) refuse(std::string("float32, bfloat16 or float16, not ") + place(x, buf));
-        if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(0)) refuse("x (..., cin) and weight (cin, cout), not " + shape(x) + " and " + shape(w));
-        const int64_t cin = w.size(0), cout = w.size(1);
-        if (cin < 1 || cin > kMost || cout > kMost) refuse("widths from 1 to 2^20, not " + std::to_string(cin) + " -> " + std::to_string(cout));
-        auto same = [&](const at::Tensor& t, const char* name) {
-            std::string b1, b2;
-            if (t.scalar_type() != x.scalar_type() || t.device() != x.device())
-                refuse(std::string(name) + " is " + place(t, b1) + ", x " + place(x, b2));
-        };
-        same(w, "weight");
-        std::vector<int64_t> out(x.sizes().begin(), x.sizes().end());
-        out.back() = cout;
-        at::Tensor b, r;
-        if (a[2] != Py_None) {
-            b = arg(a[2], "bias");
-            same(b, "bias");
-            if (b.dim() != 1 || b.size(0) != cout) refuse("bias (" + std::to_string(cout) + ",), not " + shape(b));
-            b = b.contiguous();
-        }
-        if (a[3] != Py_None) {
-            r = arg(a[3], "residual");
-            same(r, "residual");
-            if (r.sizes() != at::IntArrayRef(out)) refuse("residual of the output's shape, not " + shape(r));
-        }
-        if (x.numel() / cin > 0x7FFFFF00) refuse("at most " + std::to_string(0x7FFFFF00) + " rows");
-        if (!x.is_cuda()) refuse("tensors on the GPU, not on " + x.device().str());
-        c10::DeviceGuard guard(x.device());
-        at::Tensor y = at::empty(out, x.options().requires_grad(false)), slope;
-        const int64_t n = x.numel() / cin, ld = padded(cout, x);
-        if (keep) slope = at::empty({n, ld}, x.options().dtype(dt == INSMOS_F32 ? at::kFloat : at::kShort).requires_grad(false));
-        if (n && cout) {
-            const Rows xr = rows_of(x, cin);
-            const Weight wt = weight_of(w);
-            Rows rr{};
-            if (r.defined()) rr = rows_of(r, cout, true);
-            const size_t need = g_linear_ws(n, (int)cin, (int)cout, dt);
-            const at::Tensor ws = need ? at::empty({(int64_t)need}, x.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
-            checked(g_linear(xr.t.data_ptr(), xr.ld, wt.t.data_ptr(), wt.ld, wt.out_in, at_ptr(b), at_ptr(rr.t), rr.ld, first, act, n, (int)cin, (int)cout,
-                             dt, y.data_ptr(), cout, at_ptr(slope), ld, at_ptr(ws), need, stream_of(x)), "insmos_linear");
-        }
-        return Py_BuildValue("NN", wrap(y), wrap(slope));
-    });
-}
-// linear_backward(dy, slopes (or y) or None, x, weight, INSMOS_SLOPE_*, need_x, need_w, need_b, need_dz) -> (dx, dweight, dbias, dz), None
-// where not needed
-PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
-    return guarded([&]() -> PyObject* {
-        if (n_args != 9 || !g_backward) refuse("internal call");
-        const at::Tensor &dy = arg(a[0], "the gradient"), &x = arg(a[2], "x"), &w = arg(a[3], "weight");
-        at::Tensor slope;
-        if (a[1] != Py_None) slope = arg(a[1], "slope");
-        const int kind = (int)PyLong_AsLong(a[4]);
-        const bool need_x = PyObject_IsTrue(a[5]), need_w = PyObject_IsTrue(a[6]), need_b = PyObject_IsTrue(a[7]), need_dz = PyObject_IsTrue(a[8]);
-        const int dt = dtype_code(x.scalar_type());
-        const int64_t cin = w.size(0), cout = w.size(1), n = x.numel() / cin, ld = padded(cout, x);
-        if (dy.scalar_type() != x.scalar_type() || dy.device() != x.device()) refuse("the gradient is of another type or device than the output");
-        c10::DeviceGuard guard(x.device());
-        const auto opt = x.options().requires_grad(false);
+struct Layer { at::Tensor x, w, b, r; int act; bool first; };   // b, r: undefined where there is none
+
+// (y, slopes for the backward pass where `keep`) of a layer whose arguments are checked here
+std::pair<at::Tensor, at::Tensor> forward_of(const Layer& l, bool keep) {
+    const at::Tensor &x = l.x, &w = l.w;
+    const int dt = dtype_code(x.scalar_type());
+    std::string buf;
+    if (dt < 0) refuse(std::string("float32, bfloat16 or float16, not ") + place(x, buf));
+    if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(0)) refuse("x (..., cin) and weight (cin, cout), not " + shape(x) + " and " + shape(w));
+    const int64_t cin = w.size(0), cout = w.size(1);
+    if (cin < 1 || cin > kMost || cout > kMost) refuse("widths from 1 to 2^20, not " + std::to_string(cin) + " -> " + std::to_string(cout));
+    auto same = [&](const at::Tensor& t, const char* name) {
+        std::string b1, b2;
+        if (t.scalar_type() != x.scalar_type() || t.device() != x.device())
+            refuse(std::string(name) + " is " + place(t, b1) + ", x " + place(x, b2));
+    };
+    same(w, "weight");
+    std::vector<int64_t> out(x.sizes().begin(), x.sizes().end());
+    out.back() = cout;
+    at::Tensor b;
+    if (l.b.defined()) {
+        same(l.b, "bias");
+        if (l.b.dim() != 1 || l.b.size(0) != cout) refuse("bias (" + std::to_string(cout) + ",), not " + shape(l.b));
+        b = l.b.contiguous();
+    }
+    if (l.r.defined()) {
+        same(l.r, "residual");
+        if (l.r.sizes() != at::IntArrayRef(out)) refuse("residual of the output's shape, not " + shape(l.r));
+    }
+    if (x.numel() / cin > 0x7FFFFF00) refuse("at most " + std::to_string(0x7FFFFF00) + " rows");
+    if (!x.is_cuda()) refuse("tensors on the GPU, not on " + x.device().str());
+    c10::DeviceGuard guard(x.device());
+    const auto opt = x.options().requires_grad(false);
+    at::Tensor y = at::empty(out, opt), slope;
+    const int64_t n = x.numel() / cin, ld = padded(cout, x);
+    if (keep) slope = at::empty({n, ld}, opt.dtype(dt == INSMOS_F32 ? at::kFloat : at::kShort));
+    if (n && cout) {
+        const Rows xr = rows_of(x, cin);
         const Weight wt = weight_of(w);
-        at::Tensor dx, dw, db, dz;
-        if (need_x) dx = at::empty(x.sizes(), opt);
-        if (need_w) dw = wt.out_in ? at::empty({cout, cin}, opt) : at::empty({cin, cout}, opt);
-        if (need_b) db = at::empty({cout}, opt);
-        if (n && cout) {
-            if (need_dz) dz = at::empty({n, ld}, opt);
-            if (need_x || need_w || need_b || need_dz) {
-                const Rows d = rows_of(dy, cout), xr = rows_of(x, cin);
-                const size_t need = g_backward_ws(n, (int)cin, (int)cout, dt);
-                const at::Tensor ws = at::empty({(int64_t)need}, opt.dtype(at::kByte));
-                checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(slope), kind == INSMOS_SLOPE_STORED ? ld : cout, kind, xr.t.data_ptr(), xr.ld,
-                                   wt.t.data_ptr(), wt.ld, wt.out_in, n, (int)cin, (int)cout, dt, at_ptr(dx), cin, at_ptr(dw),
-                                   wt.out_in ? cin : cout, at_ptr(db), at_ptr(dz), ld, ws.data_ptr(), need, stream_of(x)),
-                        "insmos_linear_backward");
-            }
-            if (need_dz) dz = dz.narrow(1, 0, cout).reshape(dy.sizes());
-        } else {
-            if (need_x) dx.zero_();
-            if (need_w) dw.zero_();
-            if (need_b) db.zero_();
-            if (need_dz) dz = at::empty(dy.sizes(), opt);
+        Rows rr{};
+        if (l.r.defined()) rr = rows_of(l.r, cout, true);
+        const size_t need = g_linear_ws(n, (int)cin, (int)cout, dt);
+        const at::Tensor ws = need ? at::empty({(int64_t)need}, opt.dtype(at::kByte)) : at::Tensor();
+        checked(g_linear(xr.t.data_ptr(), xr.ld, wt.t.data_ptr(), wt.ld, wt.out_in, at_ptr(b), at_ptr(rr.t), rr.ld, l.first, l.act, n, (int)cin, (int)cout, dt,
+                         y.data_ptr(), cout, at_ptr(slope), ld, at_ptr(ws), need, stream_of(x)), "insmos_linear");
+    }
+    return {y, slope};
+}
+struct Grads { at::Tensor x, w, b, z; };
+// The gradients that are asked for (z: that of the value before the activation).  kind: INSMOS_SLOPE_*
+Grads backward_of(const at::Tensor& dy, const at::Tensor& slope, const at::Tensor& x, const at::Tensor& w, int kind, bool need_x, bool need_w, bool need_b,
+                  bool need_z) {
+    const int dt = dtype_code(x.scalar_type());
+    const int64_t cin = w.size(0), cout = w.size(1), n = x.numel() / cin, ld = padded(cout, x);
+    if (dy.scalar_type() != x.scalar_type() || dy.device() != x.device()) refuse("the gradient is of another type or device than the output");
+    c10::DeviceGuard guard(x.device());
+    const auto opt = x.options().requires_grad(false);
+    const Weight wt = weight_of(w);
+    Grads g;
+    if (need_x) g.x = at::empty(x.sizes(), opt);
+    if (need_w) g.w = wt.out_in ? at::empty({cout, cin}, opt) : at::empty({cin, cout}, opt);
+    if (need_b) g.b = at::empty({cout}, opt);
+    if (need_z) g.z = n && cout ? at::empty({n, ld}, opt) : at::empty(dy.sizes(), opt);
+    if (n && cout) {
+        if (need_x || need_w || need_b || need_z) {
+            const Rows d = rows_of(dy, cout), xr = rows_of(x, cin);
+            const size_t need = g_backward_ws(n, (int)cin, (int)cout, dt);
+            const at::Tensor ws = at::empty({(int64_t)need}, opt.dtype(at::kByte));
+            checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(slope), kind == INSMOS_SLOPE_STORED ? ld : cout, kind, xr.t.data_ptr(), xr.ld, wt.t.data_ptr(),
+                               wt.ld, wt.out_in, n, (int)cin, (int)cout, dt, at_ptr(g.x), cin, at_ptr(g.w), wt.out_in ? cin : cout, at_ptr(g.b),
+                               at_ptr(g.z), ld, ws.data_ptr(), need, stream_of(x)), "insmos_linear_backward");
         }
-        if (need_w && wt.out_in) dw = dw.t();
-        return Py_BuildValue("NNNN", wrap(dx), wrap(dw), wrap(db), wrap(dz));
+        if (need_z) g.z = g.z.narrow(1, 0, cout).reshape(dy.sizes());
+    } else {
+        for (at::Tensor* t : {&g.x, &g.w, &g.b})
+            if (t->defined()) t->zero_();
+    }
+    if (need_w && wt.out_in) g.w = g.w.t();
+    return g;
+}
+// The node keeps x, W and the activation's slopes (16 bits each with 16-bit types; y itself for relu, whose slope is its sign).
+struct LinearNode : torch::autograd::Function<LinearNode> {
+    enum : int64_t { kFirst = 4, kBias = 8, kResidual = 16 };   // beside the two bits of INSMOS_SLOPE_*
+    using Maybe = std::optional<at::Tensor>;
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const Maybe& b, const Maybe& r, int64_t act,
+                              bool first) {
+        // relu: y > 0 says what z > 0 does, unless a residual was added behind it
+        const bool of_y = act == INSMOS_ACT_RELU && (!r || first);
+        const auto out = forward_of({x, w, b.value_or(at::Tensor()), r.value_or(at::Tensor()), (int)act, first}, act != INSMOS_ACT_NONE && !of_y);
+        ctx->save_for_backward({x, w, of_y ? out.first : out.second});
+        ctx->saved_data["meta"] = (act == INSMOS_ACT_NONE ? INSMOS_SLOPE_NONE : of_y ? INSMOS_SLOPE_SIGN : INSMOS_SLOPE_STORED) + (first ? kFirst : 0) +
+                                  (b ? kBias : 0) + (r ? kResidual : 0);
+        return out.first;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dys) {
+        const bool again = at::GradMode::is_enabled();   // create_graph
+        torch::autograd::variable_list out(6);
+        try {
+            at::AutoGradMode off(false);
+            const auto saved = ctx->get_saved_variables();
+            const int64_t meta = ctx->saved_data["meta"].toInt();
+            const int kind = (int)(meta & 3);
+            // an input that is not there has no edge
+            const bool need_b = meta & kBias && ctx->needs_input_grad(2), need_r = meta & kResidual && ctx->needs_input_grad(meta & kBias ? 3 : 2);
+            const bool z = need_r && meta & kFirst && kind != INSMOS_SLOPE_NONE;
+            const Grads g = backward_of(dys[0], saved[2], saved[0], saved[1], kind, ctx->needs_input_grad(0), ctx->needs_input_grad(1), need_b, z);
+            out[0] = g.x;
+            out[1] = g.w;
+            out[2] = g.b;
+            if (need_r) out[3] = z ? g.z : dys[0];
+        } catch (const LibraryError& e) {   // the tape hands a Python error on as it is
+            PyGILState_STATE gil = PyGILState_Ensure();
+            raise("insmos_amd._lib", "InsmosHipError", e.what());
+            python_error error;
+            error.persist();
+            PyGILState_Release(gil);
+            throw error;
+        }
+        if (again) {   // a second derivative raises, and is not taken for zero
+            for (auto& t : out)
+                if (t.defined()) t = t.detach().requires_grad_(true);
+            const auto error = std::make_shared<torch::autograd::DelayedError>("linear is differentiable once: its gradients have none", (int64_t)out.size());
+            out = (*error)(std::move(out));
+        }
+        return out;
+    }
+};
+// linear(x, weight, bias or None, residual or None, act, residual_first) -> y
+PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 6 || !g_linear) refuse("internal call");
+        Layer l{arg(a[0], "x"), arg(a[1], "weight"), a[2] == Py_None ? at::Tensor() : arg(a[2], "bias"), a[3] == Py_None ? at::Tensor() : arg(a[3], "residual"),
+                (int)PyLong_AsLong(a[4]), PyObject_IsTrue(a[5]) == 1};
+        bool tape = false;
+        if (at::GradMode::is_enabled())
+            for (const at::Tensor* t : {&l.x, &l.w, &l.b, &l.r}) tape = tape || (t->defined() && t->requires_grad());
+        if (tape) {
+            auto maybe = [](const at::Tensor& t) { return t.defined() ? LinearNode::Maybe(t) : std::nullopt; };
+            return wrap(LinearNode::apply(l.x, l.w, maybe(l.b), maybe(l.r), (int64_t)l.act, l.first));
+        }
+        return wrap(forward_of(l, false).first);
     });
 }
 
 PyMethodDef kMethods[] = {{"opt_table", opt_table, METH_VARARGS, "checks lists of tensors and writes their InsmosOptTensor table"},
                           {"bind_linear", bind_linear, METH_VARARGS, "addresses of the library's functions"},
-                          {"linear_forward", (PyCFunction)(void (*)())linear_forward, METH_FASTCALL, "checks and insmos_linear"},
-                          {"linear_backward", (PyCFunction)(void (*)())linear_backward, METH_FASTCALL, "insmos_linear_backward"},
+                          {"linear", (PyCFunction)(void (*)())linear, METH_FASTCALL, "the layer, on the autograd tape"},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 }  // namespace
