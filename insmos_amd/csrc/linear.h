@@ -108,16 +108,25 @@ template <> struct Slope<float> {
     static __device__ __forceinline__ float store(float s) { return s; }
     static __device__ __forceinline__ float load(float s) { return s; }
 };
+// eight values of a row from i on, of which `left` > 0 exist (behind them: the last one again); and the first `left` of eight stored
 template <class T>
-__device__ __forceinline__ f32x8 load8(const void* q, int64_t i) { return __builtin_convertvector(*(const typename Mem8<T>::t*)((const T*)q + i), f32x8); }
-template <class T>
-__device__ __forceinline__ void store8(void* q, int64_t i, f32x8 v) {
+__device__ __forceinline__ typename Mem8<T>::t load8(const void* q, int64_t i, int left) {
     typedef typename Mem8<T>::t M8;
-    *(M8*)((T*)q + i) = __builtin_convertvector(v, M8);
+    if (left >= 8) return *(const M8*)((const T*)q + i);
+    M8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = ((const T*)q)[i + min(e, left - 1)];
+    return v;
 }
-// values n..n+7 of row m from the fp32 sums, all inside the matrix; b and r: bias and residual (zeros where there is none)
+template <class V>
+__device__ __forceinline__ f32x8 wide(V v) { return __builtin_convertvector(v, f32x8); }
+// Values n..n+7 (n < N) of row m from the fp32 sums; b and r: bias and residual (zeros where there is none).  Columns behind N are computed with
+// the rest and not stored: only loads and stores differ at the edge (a second, one by one epilogue there held up 4099 x 1000 x 1533 fp16 by 16
+// of 53 us, as the last tile column was on its own with it).
 template <class T>
 __device__ __forceinline__ void epilogue8(const GemmP& p, int m, int n, f32x8 v, f32x8 b, f32x8 r) {
+    typedef typename Mem8<T>::t M8;
+    const int left = p.N - n;
     v += b;
     if (p.res_first) v += r;
     float s;
@@ -130,36 +139,33 @@ __device__ __forceinline__ void epilogue8(const GemmP& p, int m, int n, f32x8 v,
             v[e] = activate(v[e], p.act, s);
             c[e] = Slope<T>::store(s);
         }
-        *(S8*)((S*)p.slope + m * p.ld_slope + n) = c;
+        S* q = (S*)p.slope + m * p.ld_slope + n;
+        if (n + 8 <= p.ld_slope) {   // (the row's rest up to 16 bytes may be written)
+            *(S8*)q = c;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) q[e] = c[e];
+        }
     } else if (p.act) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = activate(v[e], p.act, s);
     }
     if (!p.res_first) v += r;
-    store8<T>(p.y, m * p.ld_y + n, v);
-}
-// the same one by one, up to the matrix's edge
-template <class T>
-__device__ __forceinline__ void epilogue1(const GemmP& p, int m, int n, f32x8 v) {
+    const M8 o = __builtin_convertvector(v, M8);
+    T* y = (T*)p.y + m * p.ld_y + n;
+    if (left >= 8) {
+        *(M8*)y = o;
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if (n + e >= p.N) break;
-        float u = v[e];
-        if (p.bias) u += (float)((const T*)p.bias)[n + e];
-        const float r = p.res ? (float)((const T*)p.res)[m * p.ld_res + n + e] : 0.f;
-        if (p.res_first) u += r;
-        float s = 1.f;
-        if (p.act) u = activate(u, p.act, s);
-        if (p.slope) ((typename Slope<T>::t*)p.slope)[m * p.ld_slope + n + e] = Slope<T>::store(s);
-        if (!p.res_first) u += r;
-        ((T*)p.y)[m * p.ld_y + n + e] = (T)u;
+        for (int e = 0; e < 8; ++e)
+            if (e < left) y[e] = o[e];
     }
 }
 template <class T>
 __device__ __forceinline__ void epilogue(const GemmP& p, int m, int n, f32x8 v) {
-    if (n + 8 > p.N) return epilogue1<T>(p, m, n, v);
     const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    epilogue8<T>(p, m, n, v, p.bias ? load8<T>(p.bias, n) : zero, p.res ? load8<T>(p.res, m * p.ld_res + n) : zero);
+    epilogue8<T>(p, m, n, v, p.bias ? wide(load8<T>(p.bias, n, p.N - n)) : zero, p.res ? wide(load8<T>(p.res, m * p.ld_res + n, p.N - n)) : zero);
 }
 
 // ---- operands ---------------------------------------------------------------------------------------------------------------
@@ -358,17 +364,17 @@ struct Gemm {
         typedef typename Mem8<T>::t M8;
         LIN_LDS char* t = turn + wave * (32 * CH * 16);
         const int n = it.tn * BN + (wave % WN) * (BN / WN) + (lane % LPR) * 8;
-        const bool whole = n + 8 <= p.N;
+        const bool in = n < p.N, plain = p.splits == 1;
         const f32x8 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const f32x8 bias = p.bias && whole && p.splits == 1 ? load8<T>(p.bias, n) : zero;
+        const f32x8 bias = p.bias && in && plain ? wide(load8<T>(p.bias, n, p.N - n)) : zero;
         float* part = p.part + (int64_t)it.split * p.M * p.ld_part;   // (ld_part: whole groups of 8)
 #pragma unroll 1
         for (int i = 0; i < TM; ++i) {
             const int m0 = it.tm * BM + (wave / WN) * (BM / WM) + i * 32 + lane / LPR;
             M8 res[PASSES];   // all of the block's residual is asked for before the first of it is needed
-            if (p.res && p.splits == 1 && whole) {
+            if (p.res && in && plain) {
 #pragma unroll
-                for (int q = 0; q < PASSES; ++q) res[q] = *(const M8*)((const T*)p.res + min(m0 + q * RPP, p.M - 1) * p.ld_res + n);
+                for (int q = 0; q < PASSES; ++q) res[q] = load8<T>(p.res, min(m0 + q * RPP, p.M - 1) * p.ld_res + n, p.N - n);
             }
             const int r = lane & 31;
 #pragma unroll
@@ -391,12 +397,10 @@ struct Gemm {
                 const f32x4 hi = *(const LIN_LDS f32x4*)(t + (row * CH + ((c + 1) ^ (row & (CH - 1)))) * 16);
                 const f32x8 v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 if (m < p.M) {
-                    if (p.splits > 1) {
+                    if (!plain) {
                         if (n < p.ld_part) *(f32x8*)(part + m * p.ld_part + n) = v;
-                    } else if (whole) {
-                        epilogue8<T>(p, m, n, v, bias, p.res ? __builtin_convertvector(res[q], f32x8) : zero);
-                    } else if (n < p.N) {
-                        epilogue1<T>(p, m, n, v);
+                    } else if (in) {
+                        epilogue8<T>(p, m, n, v, bias, p.res ? wide(res[q]) : zero);
                     }
                 }
             }
