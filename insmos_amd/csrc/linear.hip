@@ -71,7 +71,7 @@ Plan plan_for(int M, int N, int K, int dtype, bool xw) {   // xw: the first oper
     // (one workgroup per 32 columns walks all of k: 16 x 8192 x 256 takes 25 us that way and 10 in parts)
     if (M <= 32 && xw && (K <= 4096 || N >= 4096)) return {FEW, 1};
     struct Shape { int tile, bm, bn, slots; double rate, rate32, fixed; };
-    static const Shape shapes[] = {{T256, 256, 256, 256, 1250, 0, 6},     {T128, 128, 128, 512, 1050, 140, 8},    {T128X64, 128, 64, 768, 800, 135, 5},
+    static const Shape shapes[] = {{T256, 256, 256, 256, 1250, 0, 12},     {T128, 128, 128, 512, 1050, 140, 8},    {T128X64, 128, 64, 768, 800, 135, 5},
                                    {T64X128, 64, 128, 768, 800, 135, 5},  {T128X32, 128, 32, 1024, 500, 120, 3}, {T32X128, 32, 128, 1024, 500, 120, 3}};
     static const int parts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512, 768, 1024};
     Plan best = {T128, 1};
