@@ -213,15 +213,22 @@ struct Tile {
         p += kt0 * step;
         left -= kt0 * step;
     }
-    // k_left: K minus the tile's first k
-    __device__ __forceinline__ void load(LIN_LDS char* __restrict lds, int k_left, int wave) {
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)max((int64_t)0, min(left, (int64_t)0x7FFFFFFF)), 0x00027000);
-        const uint32_t v = LAY == KC && chunk >= k_left ? 0x80000000u : voff;
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (LIN_LDS void*)(lds + (i * NW + wave) * 1024), 16, v, i * istep, 0, 0);
+    // The loads of the current k tile: where from (k_left: K minus the tile's first k; without `on` nothing is read), and instruction i.
+    struct Source { __amdgpu_buffer_rsrc_t rs; uint32_t v; };
+    __device__ __forceinline__ Source source(int k_left, bool on = true) {
+        const int bytes = on ? (int)max((int64_t)0, min(left, (int64_t)0x7FFFFFFF)) : 0;
+        const Source r = {__builtin_amdgcn_make_buffer_rsrc((void*)p, 0, bytes, 0x00027000), LAY == KC && chunk >= k_left ? 0x80000000u : voff};
         p += step;
         left -= step;
+        return r;
+    }
+    __device__ __forceinline__ void load1(const Source& f, LIN_LDS char* __restrict lds, int i, int wave) const {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(f.rs, (LIN_LDS void*)(lds + (i * NW + wave) * 1024), 16, f.v, i * istep, 0, 0);
+    }
+    __device__ __forceinline__ void load(LIN_LDS char* __restrict lds, int k_left, int wave) {   // all of them
+        const Source f = source(k_left);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) load1(f, lds, i, wave);
     }
     // KC: the chunk that K ends in has brought values from behind the row's end; zeros in their place (k: valid values of the tile)
     static __device__ __forceinline__ void cut(LIN_LDS char* lds, int k) {
@@ -339,20 +346,40 @@ struct Gemm {
     }
     static __device__ __forceinline__ void step(LIN_LDS char* __restrict wr, const LIN_LDS char* __restrict rd, TA& ta, TB& tb, const FA& fa,
                                                 const FB& fb, Regs& r, f32x16 (&acc)[TM][TN], bool more, int k_left, int wave) {
-        if (more) {
-            ta.load(wr, k_left, wave);
-            tb.load(wr + SA, k_left, wave);
-        }
+        if constexpr (sizeof(T) == 2) {
+            if (more) {
+                ta.load(wr, k_left, wave);
+                tb.load(wr + SA, k_left, wave);
+            }
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            phase(rd, fa, fb, r, acc, s);
-            if (sizeof(T) == 2) {
+            for (int s = 0; s < 4; ++s) {
+                phase(rd, fa, fb, r, acc, s);
                 // reads and matrix instructions in turn, and not the reads in a row in front (1096 -> 1255 TFLOP/s at 8192 x 8192 x 4096, bf16,
                 // with the phases' overlap across the barrier)
 #pragma unroll
                 for (int q = 0; q < TM * TN; ++q) {
                     __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);   // LDS reads
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // one matrix instruction
+                }
+            }
+        } else {
+            // The loads between the matrix instructions of PH phases (in front, a wave that waits for a place in the load queue holds its matrix
+            // unit up: 4096 x 4096 x 4096 fp32 1010 -> 980 us; with 16 bits, whose steps are a quarter as long, it is the other way round).
+            constexpr int PH = 2, LOADS = TA::NI + TB::NI, EACH = (LOADS + PH - 1) / PH, GAP = TM * TN * 4 / EACH;
+            const typename TA::Source sa = ta.source(k_left, more);
+            const typename TB::Source sb = tb.source(k_left, more);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int i = s * EACH; i < LOADS && i < (s + 1) * EACH; ++i) {
+                    if (i < TA::NI) ta.load1(sa, wr, i, wave);
+                    else tb.load1(sb, wr + SA, i - TA::NI, wave);
+                }
+                phase(rd, fa, fb, r, acc, s);
+#pragma unroll
+                for (int i = s * EACH; i < LOADS && i < (s + 1) * EACH; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);     // a load
+                    __builtin_amdgcn_sched_group_barrier(0x008, GAP, 0);   // matrix instructions
                 }
             }
         }
