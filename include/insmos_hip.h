@@ -859,7 +859,8 @@ int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dt
  * Backward: dz = dy act'(z);  dx = dz W^T;  dw = x^T dz in the weight's layout;  db = column sums of dz (before its rounding to the type).
  * slope_kind: INSMOS_SLOPE_NONE (no activation), INSMOS_SLOPE_SIGN (slope holds y = relu(z), of which the sign counts) or INSMOS_SLOPE_STORED.
  * Each of dx, dw, db, dz may be NULL; dz: 16-byte aligned rows like slope's.
- * ws: 16-byte aligned, insmos_linear*_ws_bytes bytes.  M = 0 is no work for insmos_linear and refused by the backward.
+ * ws: 16-byte aligned, insmos_linear*_ws_bytes bytes.  M = 0 is no work for insmos_linear and refused by the backward.  Outputs overlap
+ * neither inputs nor each other.
  * ---------------------------------------------------------------------------------------------- */
 #define INSMOS_ACT_NONE 0
 #define INSMOS_ACT_RELU 1

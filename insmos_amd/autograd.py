@@ -1,4 +1,4 @@
-"""Training-step building blocks on MI355X (SURVEY.md 8f rank 2 -- a FIRST SLICE, see include/insmos_hip.h):
+"""Training-step building blocks on MI355X (C side: include/insmos_hip.h):
 
   * SparseConvFunction / sparse_conv(): the output-stationary sparse convolution as a torch.autograd.Function whose
     forward AND backward are HIP kernels -- d/dx is the same MFMA kernel on the transposed table with transposed taps,
@@ -10,7 +10,8 @@ torch is used for what it is here for -- device memory, streams and the autograd
 (models/models.py:61-98 calls loss.backward() on such a tape).
   * batch_norm_train(): nn.BatchNorm1d / MinkowskiBatchNorm in train() mode (+ fused ReLU), forward and backward.
   * center_assign_targets() / center_head_loss(): CenterHead.assign_targets / get_loss (center_head.py:126-331).
-The optimiser step stays torch.optim's.
+  * linear(): a pointwise layer (1x1 convolution, nn.Linear) with bias, activation and residual in the product's epilogue.
+The optimiser step is optim.py's, or torch.optim's.
 """
 import contextlib
 import ctypes
@@ -511,7 +512,8 @@ def linear(x, weight, bias=None, residual=None, activation=None, residual_first=
     .t()) is read as it lies.  bias (cout,).  residual: the output's shape (an expanded one works: rows of pitch 0).  activation: None,
     "relu", "gelu" (erf), "gelu_tanh" or "silu".  All tensors of one dtype -- float32, bfloat16 or float16 -- on one GPU; sums in fp32.
     Widths up to 2^20.  Differentiable once in all four tensors; without gradients nothing is kept for a backward pass.  In 16 bits the
-    backward rounds dz once, for the products."""
+    backward rounds dz once, for the products.  Forward and backward can be captured into a graph; the backward refuses where a graph that
+    was recorded on the default stream shares its inputs and is still alive."""
     try:
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):

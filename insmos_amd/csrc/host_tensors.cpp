@@ -7,6 +7,7 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -59,6 +60,27 @@ const at::Tensor& tensor_at(PyObject* list, Py_ssize_t i, const char* what, cons
 }
 int dtype_code(c10::ScalarType t) {
     return t == c10::ScalarType::Float ? INSMOS_F32 : t == c10::ScalarType::BFloat16 ? INSMOS_BF16 : t == c10::ScalarType::Half ? INSMOS_F16 : -1;
+}
+
+// opt_order(params) -> a hash of the tensors' sizes and strides
+PyObject* opt_order(PyObject*, PyObject* list) {
+    if (!PyList_Check(list)) { PyErr_SetString(PyExc_ValueError, "opt_order: params is a list"); return nullptr; }
+    uint64_t h = 0xCBF29CE484222325u;
+    auto add = [&](int64_t v) { h = (h ^ (uint64_t)v) * 0x100000001B3u; };
+    try {
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+            const at::Tensor& t = tensor_at(list, i, "opt_order", "parameter");
+            add(t.dim());
+            for (int64_t d = 0; d < t.dim(); ++d) {
+                add(t.size(d));
+                add(t.stride(d));
+            }
+        }
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_ValueError, e.what());
+        return nullptr;
+    }
+    return PyLong_FromUnsignedLongLong(h);
 }
 
 // opt_table(what, params or None, grads, table, any_device) -> (entries, dtype code, length of the state buffers, gradients to reorder)
@@ -302,6 +324,18 @@ Grads backward_of(const at::Tensor& dy, const at::Tensor& slope, const at::Tenso
     if (need_w && wt.out_in) g.w = g.w.t();
     return g;
 }
+// A backward pass that is captured into a graph must not reach a node that was recorded on the default stream (a leaf's, kept alive by an eager
+// graph): the tape would make that stream wait for the captured one, which cannot be captured and ends the process.
+void refuse_default_stream() {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto node = torch::autograd::get_current_node();
+    if (!node) return;
+    for (const auto& edge : node->next_edges()) {
+        const auto stream = edge.function ? edge.function->stream() : std::nullopt;
+        if (stream && stream->id() == 0)
+            refuse("a backward pass is being captured, but a graph on the default stream shares its inputs and is alive (drop that graph's outputs before the capture)");
+    }
+}
 // The node keeps x, W and the activation's slopes (16 bits each with 16-bit types; y itself for relu, whose slope is its sign).
 struct LinearNode : torch::autograd::Function<LinearNode> {
     enum : int64_t { kFirst = 4, kBias = 8, kResidual = 16 };   // beside the two bits of INSMOS_SLOPE_*
@@ -321,6 +355,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         torch::autograd::variable_list out(6);
         try {
             at::AutoGradMode off(false);
+            refuse_default_stream();
             const auto saved = ctx->get_saved_variables();
             const int64_t meta = ctx->saved_data["meta"].toInt();
             const int kind = (int)(meta & 3);
@@ -366,7 +401,8 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     });
 }
 
-PyMethodDef kMethods[] = {{"opt_table", opt_table, METH_VARARGS, "checks lists of tensors and writes their InsmosOptTensor table"},
+PyMethodDef kMethods[] = {{"opt_order", opt_order, METH_O, "a hash of sizes and strides"},
+                          {"opt_table", opt_table, METH_VARARGS, "checks lists of tensors and writes their InsmosOptTensor table"},
                           {"bind_linear", bind_linear, METH_VARARGS, "addresses of the library's functions"},
                           {"linear", (PyCFunction)(void (*)())linear, METH_FASTCALL, "the layer, on the autograd tape"},
                           {nullptr, nullptr, 0, nullptr}};

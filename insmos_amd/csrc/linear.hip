@@ -16,21 +16,21 @@ size_t size_of(int dtype) { return dtype == INSMOS_F32 ? 4 : 2; }
 // The tile loads move 16 bytes from any address on 4 bytes; 16-bit operands at odd addresses or pitches are copied into rows padded with zeros.
 __global__ void __launch_bounds__(256) k_linear_pack(const uint16_t* __restrict__ src, int64_t ld, int64_t rows, int cols, uint16_t* __restrict__ dst,
                                                      int ld_dst) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     constexpr int V = 8;
     const int per = ld_dst / V;
-    const int64_t r = i / per;
-    const int c = (int)(i % per) * V;
-    if (r >= rows) return;
-    typedef uint16_t U8 __attribute__((ext_vector_type(8), aligned(2)));
-    U8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (c + V <= cols) v = *(const U8*)(src + r * ld + c);
-    else
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per;
+        const int c = (int)(i % per) * V;
+        typedef uint16_t U8 __attribute__((ext_vector_type(8), aligned(2)));
+        U8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (c + V <= cols) v = *(const U8*)(src + r * ld + c);
+        else
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-            if (c + e < cols) v[e] = src[r * ld + c + e];
-    typedef uint16_t A8 __attribute__((ext_vector_type(8)));
-    *(A8*)(dst + r * ld_dst + c) = v;
+            for (int e = 0; e < V; ++e)
+                if (c + e < cols) v[e] = src[r * ld + c + e];
+        typedef uint16_t A8 __attribute__((ext_vector_type(8)));
+        *(A8*)(dst + r * ld_dst + c) = v;
+    }
 }
 struct Operand {
     const void* p;
@@ -49,9 +49,8 @@ int operand(const void* p, int64_t ld, int64_t rows, int cols, int lay, int dtyp
     const int es = (int)size_of(dtype), to = round_up(cols, 16 / es);
     char* d = ws.take<char>((size_t)rows * to * es);
     if (!d) return INSMOS_EWORKSPACE;
-    const int64_t threads = rows * (to / (16 / es));
-    if ((threads + 255) / 256 > 0x7FFFFFFF / 256) return INSMOS_EINVAL;
-    const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+    const int64_t groups = (rows * (to / (16 / es)) + 255) / 256;
+    const dim3 grid((unsigned)(groups < 1 << 22 ? groups : 1 << 22)), block(256);
     INSMOS_LAUNCH(k_linear_pack, grid, block, 0, s, (const uint16_t*)p, ld, rows, cols, (uint16_t*)d, to);
     HIP_TRY(hipGetLastError());
     *out = {d, to, lay};
@@ -63,8 +62,8 @@ struct Plan { int tile, splits; };
 // Up to 32 rows (x W alone) there is a kernel of its own.  Otherwise the tile and the number of parts of k with the shortest predicted time:
 //   rounds of the workgroups that fit on the chip, each k tiles x max(0.75 us, workgroups per CU x a tile's work at the CU's rate) + a fixed
 //   part for its first loads and its epilogue; with parts, their bytes at 4 TB/s and another launch.
-// Rates (all CUs together, TFLOP/s) and fixed parts (us) are measured; predicted / measured, us, bf16: 8192 x 1024 x 1024 128x128 24 / 24,
-// 256x256 34 / 32; 2048^3 128x64 29 / 26, 128x128 32 / 31; 512 x 4096 x 512 128x64 in 8 parts 18 / 15, 128x128 in 16 23 / 21; fp32:
+// Rates (all CUs together, TFLOP/s) and fixed parts (us) are measured; predicted / measured, us, bf16: 8192 x 1024 x 1024 128x128 24 / 26,
+// 256x256 39 / 33; 2048^3 128x64 29 / 32, 128x128 32 / 35; 512 x 4096 x 512 128x64 in 8 parts 18 / 15, 128x128 in 16 23 / 21; fp32:
 // 300000 x 128 x 256 128x128 234 / 231, 128x64 212 / 213; 119817 x 64 x 128 128x128 31 / 37, 128x32 29 / 33.
 Plan plan_for(int M, int N, int K, int dtype, bool xw) {   // xw: the first operand has contiguous k
     const int bk = 128 / (int)size_of(dtype), nk = (K + bk - 1) / bk;

@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(1024) k_adamw_prepare(const PrepareP A) {
     if (threadIdx.x > 1) return;
     if (A.norm_in) norm = (double)*A.norm_in;
     StepVals v;
-    v.skip = A.skip_nonfinite && !(norm <= 1.7976931348623157e308);
+    v.skip = A.skip_nonfinite && !((float)norm <= 3.402823466e38f);   // (what norm_out says)
     const int t = *A.step + (v.skip ? 0 : 1);
     const double power = pow(threadIdx.x ? A.b2 : A.b1, (double)t), power2 = __shfl(power, 1);   // lane 0: b1^t, lane 1: b2^t
     if (threadIdx.x) return;

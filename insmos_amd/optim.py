@@ -15,6 +15,7 @@ Nothing is read back from the device and no memory is kept between calls of the 
 captured step repeats with the addresses of the tensors it was captured with and the learning rate it was captured with unless that
 is a tensor.
 """
+import collections
 import ctypes
 import math
 
@@ -113,6 +114,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, *, lr, betas=(0.9, 0.99
     state = torch.float8_e4m3fn if bits == 8 else torch.float32
     _flat("exp_avg", exp_avg, state, total, dev)
     _flat("exp_avg_sq", exp_avg_sq, state, total, dev)
+    if total and abs(exp_avg.data_ptr() - exp_avg_sq.data_ptr()) < total * exp_avg.element_size():
+        raise ValueError("adamw_step: exp_avg and exp_avg_sq share memory")
     if bits == 8:
         if scales is None:
             raise ValueError("adamw_step: moments in 8 bits need scales")
@@ -164,6 +167,8 @@ class _Bucket:
     def __init__(self, params, state_bits, master_weights):
         self.params = params
         dev, dtype = params[0].device, params[0].dtype
+        from . import _host
+        self.order = _host.opt_order(params)
         self.starts, total = state_offsets([p.numel() for p in params])
         state = torch.float8_e4m3fn if state_bits == 8 else torch.float32
         self.exp_avg, self.exp_avg_sq = (torch.zeros(total, dtype=torch.float32, device=dev).to(state) for _ in range(2))
@@ -174,6 +179,12 @@ class _Bucket:
             self.masters = torch.zeros(total, dtype=torch.float32, device=dev)
             for i in range(len(params)):
                 self.view(self.masters, i).copy_(params[i].detach())
+
+    def __getstate__(self):     # (the codes as bytes: torch pickles no 8-bit floats)
+        return {k: v.view(torch.uint8) if torch.is_tensor(v) and v.dtype == torch.float8_e4m3fn else v for k, v in self.__dict__.items()}
+
+    def __setstate__(self, state):
+        self.__dict__.update({k: v.view(torch.float8_e4m3fn) if torch.is_tensor(v) and v.dtype == torch.uint8 else v for k, v in state.items()})
 
     def view(self, flat, i):
         """Tensor i's part of a state buffer, shaped and ordered as the parameter."""
@@ -194,13 +205,14 @@ class _Bucket:
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled=False: Adam with the decay in the gradient) whose step() is adamw_step() on every parameter group.
 
-    state_bits: 32, or 8 (4 bytes less than half a byte over 2 per parameter instead of 8).  master_weights: keep fp32 weights of
+    state_bits: 32, or 8 (two bytes of moments per parameter and 8 more per 256, instead of eight per parameter).  master_weights: keep fp32 weights of
     bfloat16 / float16 parameters.  max_grad_norm: clip by the norm over ALL gradients of the optimiser.  skip_nonfinite: a step whose
     gradients' norm is inf or NaN changes nothing.  seed: of the 8-bit rounding.  lr may be a float32 tensor on the device (a captured
     step then follows it).  After step(), last_grad_norm holds the norm (None where it was not taken).
 
     A group's parameters share one step counter; a parameter without a gradient keeps its value and moments.  The state is made at the
-    first step (or load_state_dict) from the parameters as they are then, and a group's list is fixed from then on."""
+    first step (or load_state_dict) from the parameters as they are then; a group's list, its shapes and their order in memory are fixed
+    from then on.  A captured step needs one that was taken before the capture."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, decoupled=True, state_bits=32,
                  master_weights=False, max_grad_norm=None, skip_nonfinite=False, seed=0):
@@ -218,6 +230,8 @@ class AdamW(torch.optim.Optimizer):
 
     def _group_buckets(self, gi):
         if gi not in self._buckets:
+            if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: the state is made by the first step, which cannot be captured (a replay would clear it)")
             lists = {}
             for p in self.param_groups[gi]["params"]:
                 lists.setdefault((p.device, p.dtype), []).append(p)
@@ -229,6 +243,7 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        from . import _host
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -236,6 +251,8 @@ class AdamW(torch.optim.Optimizer):
         work = []
         for gi, group in enumerate(self.param_groups):
             for b in self._group_buckets(gi):
+                if _host.opt_order(b.params) != b.order:
+                    raise RuntimeError("AdamW: a parameter's shape or order in memory has changed since its state was made")
                 grads = [p.grad for p in b.params]
                 if any(g is not None for g in grads):
                     work.append((group, b, grads))
@@ -249,6 +266,18 @@ class AdamW(torch.optim.Optimizer):
                                 max_grad_norm=self.max_grad_norm, grad_norm=norm, skip_nonfinite=self.skip_nonfinite, seed=self.seed)
         self.last_grad_norm = norm_b if work and wanted else None
         return loss
+
+    _KEPT = ("state_bits", "master_weights", "max_grad_norm", "skip_nonfinite", "seed", "last_grad_norm", "_buckets")
+
+    def __getstate__(self):     # (copies and pickles; the entries of self.state are views of the buffers, made again)
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in self._KEPT}, "state": collections.defaultdict(dict)}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for bs in self._buckets.values():
+            for b in bs:
+                for i, p in enumerate(b.params):
+                    self.state[p] = b.entries(i)
 
     def load_state_dict(self, state_dict):
         """A state_dict() of an AdamW with the same state_bits and master_weights over parameters of the same shapes."""

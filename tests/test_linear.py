@@ -367,3 +367,35 @@ def test_linear_entry_points_refuse():
                 {"dz": p + 4}, {"dz": p, "lddz": 15}, {"dt": -1}, {"ldd": 15}):
         assert backward(**bad) == -1, bad
     assert backward(kind=1, slope=p, n=0) == -3      # dz needs room
+
+
+@pytest.mark.gpu
+def test_linear_captured_beside_a_live_eager_graph():
+    """An eager graph on the default stream keeps its leaves' nodes: a backward pass that is captured on another stream would reach them, and is
+    refused.  Once that graph is gone the same capture works and replays what an eager pass gives."""
+    gen = torch.Generator().manual_seed(31)
+    x, gy = torch.randn(37, 24, generator=gen).cuda(), torch.randn(37, 16, generator=gen).cuda()
+    w = (torch.randn(24, 16, generator=gen) * 0.3).cuda().requires_grad_(True)
+    alive = linear(x, w, activation="silu")
+    (want,) = torch.autograd.grad(alive, w, gy, retain_graph=True)
+    torch.cuda.synchronize()
+
+    def capture():
+        g, out = torch.cuda.CUDAGraph(), None
+        with torch.cuda.graph(g):
+            try:
+                (out,) = torch.autograd.grad(linear(x, w, activation="silu"), w, gy)
+            except RuntimeError as e:
+                out = str(e)
+        return g, out
+
+    _, said = capture()
+    assert isinstance(said, str) and "being captured" in said
+    del alive
+    g, out = capture()
+    assert torch.is_tensor(out), out
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)

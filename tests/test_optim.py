@@ -567,3 +567,77 @@ def test_entry_points_refuse():
     assert lib.insmos_grad_sumsq_partials(at, 1) == 3
     assert lib.insmos_grad_sumsq(at, 1, 0, p, 2, None) == -3 and lib.insmos_grad_sumsq(at, 1, 0, None, 3, None) == -1 and lib.insmos_grad_sumsq(at, 1, 9, p, 3, None) == -1
     assert lib.insmos_grad_norm(None, 1, p, None) == -1 and lib.insmos_grad_norm(p, 1, None, None) == -1
+
+
+@pytest.mark.gpu
+def test_a_norm_beyond_float32_is_not_finite():
+    """Two gradients of 3e38: their norm, 4.2e38, is above float32's largest number (3.4e38), so norm_out says inf and the step is left out."""
+    for bits in (32, 8):
+        p = torch.ones(600, device="cuda")
+        g = torch.zeros(600, device="cuda")
+        g[:2] = 3e38
+        m, v = (torch.zeros(768, device="cuda").to(torch.float32 if bits == 32 else torch.float8_e4m3fn) for _ in range(2))
+        step = torch.zeros(1, dtype=torch.int32, device="cuda")
+        norm = adamw_step([p], [g], m, v, step, lr=0.1, skip_nonfinite=True, scales=None if bits == 32 else torch.zeros(2, 3, device="cuda"))
+        assert norm.item() == float("inf") and step.item() == 0 and torch.equal(p, torch.ones_like(p))
+        g[1] = 0.0
+        assert adamw_step([p], [g], m, v, step, lr=0.1, skip_nonfinite=True, max_grad_norm=1.0,
+                          scales=None if bits == 32 else torch.zeros(2, 3, device="cuda")).item() == torch.tensor(3e38).item()
+        assert step.item() == 1 and p[0].item() != 1.0
+
+
+@pytest.mark.gpu
+def test_moments_in_one_buffer_are_refused():
+    p, g, m = (torch.ones(300, device="cuda") for _ in range(3))
+    buf, step = torch.zeros(1024, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    for a, b in ((buf[:512], buf[:512]), (buf[:512], buf[256:768]), (buf[256:768], buf[:512])):
+        with pytest.raises(ValueError, match="share memory"):
+            adamw_step([p], [g], a, b, step, lr=0.1)
+    adamw_step([p], [g], buf[:512], buf[512:], step, lr=0.1)
+    assert step.item() == 1
+
+
+@pytest.mark.gpu
+def test_optimizer_refuses_changed_parameters_and_a_captured_first_step():
+    p = torch.nn.Parameter(torch.randn(4, 8, 3, 3, device="cuda"))
+    p.grad = torch.randn_like(p)
+    o = AdamW([p], lr=0.1)
+    said, stream = None, torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        try:
+            o.step()
+        except RuntimeError as e:
+            said = str(e)
+    assert "captured" in said and not o.state
+    o.step()
+    p.data = p.data.to(memory_format=torch.channels_last)
+    with pytest.raises(RuntimeError, match="order in memory"):
+        o.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_copies_and_pickles(bits):
+    """A copy (deepcopy, pickle) with its parameters goes on as the original does, and its state entries are views of its own buffers."""
+    import copy
+    import pickle
+    gen = torch.Generator().manual_seed(5)
+    ps = [torch.nn.Parameter(torch.randn(s, generator=gen).cuda()) for s in ((7, 5), (300,), (3, 4, 2))]
+    o = AdamW(ps, lr=0.01, state_bits=bits, max_grad_norm=1.0, seed=9)
+    gs = [[torch.randn(p.shape, generator=gen).cuda() for p in ps] for _ in range(4)]
+
+    def go(opt, its):
+        for it in its:
+            for p, g in zip(opt.param_groups[0]["params"], gs[it]):
+                p.grad = g.clone()
+            opt.step()
+        return [p.detach().clone() for p in opt.param_groups[0]["params"]]
+
+    go(o, range(2))
+    copies = [copy.deepcopy(o), pickle.loads(pickle.dumps(o))]
+    want = go(o, range(2, 4))
+    for c in copies:
+        assert all(torch.equal(a, b) for a, b in zip(go(c, range(2, 4)), want))
+        for p, q in zip(c.param_groups[0]["params"], ps):
+            assert all(torch.equal(c.state[p][k].float(), o.state[q][k].float()) for k in o.state[q])
