@@ -399,3 +399,12 @@ def test_linear_captured_beside_a_live_eager_graph():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("M,K,N", [(4090, 2100, 4090), (4000, 300, 1901), (2050, 8200, 2050), (61, 700, 30002), (8200, 520, 2055)])
+def test_linear_large_tiles(M, K, N, dtype):
+    """Sizes that take the 256 x 256 tile (whole and with k in parts), the 128 x 128 one and 64 and 32 rows of it, each with partial last tiles."""
+    for layout in ("in_out", "out_in"):
+        _check(*_case(M, K, N, dtype, "gelu_tanh", True, layout, seed=8), "gelu_tanh", False)
