@@ -119,6 +119,7 @@ struct SlopeP {
     const void* slope;   // INSMOS_SLOPE_SIGN: y; INSMOS_SLOPE_STORED: what the forward stored
     void* dz;            // or null: column sums alone
     float* part;         // [row blocks][ld_part] or null
+    void* db;            // one row block: the sums' place, in the type, or null
     int64_t ld_dy, ld_slope, ld_dz;
     int64_t M;
     int N, ld_part, kind, rows;   // rows per workgroup
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {
             }
         }
     }
-    if (!p.part) return;
+    if (!p.part && !p.db) return;
     __shared__ float s[256][V + 1];
 #pragma unroll
     for (int e = 0; e < V; ++e) s[threadIdx.x][e] = sum[e];
@@ -198,7 +199,10 @@ __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {
     if (r0 == 0) {
 #pragma unroll
         for (int e = 0; e < V; ++e)
-            if (n + e < p.N) p.part[(int64_t)blockIdx.y * p.ld_part + n + e] = s[threadIdx.x][e];
+            if (n + e < p.N) {
+                if (p.db) ((T*)p.db)[n + e] = (T)s[threadIdx.x][e];
+                else p.part[(int64_t)blockIdx.y * p.ld_part + n + e] = s[threadIdx.x][e];
+            }
     }
 }
 // db[n] = sum over the row blocks: 64 lanes per column, then a tree
@@ -231,7 +235,7 @@ SlopePlan slope_plan(int64_t M, int N, int dtype) {
     int64_t blocks = 2048 / r.strips;
     if (blocks < 1) blocks = 1;
     int64_t rows = ((M + blocks - 1) / blocks + step - 1) / step * step;
-    const int64_t least = 4 * step;
+    const int64_t least = 8 * step;   // (two trips of four rows in flight)
     if (rows < least) rows = least;
     if (rows > (int64_t)1 << 30) rows = (int64_t)1 << 30;
     r.rows = (int)rows;
@@ -244,7 +248,7 @@ int run_slope_t(const SlopeP& p, const SlopePlan& r, void* db, hipStream_t s) {
                         : p.kind == INSMOS_SLOPE_SIGN ? k_linear_slope<T, INSMOS_SLOPE_SIGN> : k_linear_slope<T, INSMOS_SLOPE_NONE>;
     INSMOS_LAUNCH(kernel, dim3(r.strips, r.blocks), dim3(256), 0, s, p);
     HIP_TRY(hipGetLastError());
-    if (db) {
+    if (p.part) {
         const auto sum = k_linear_colsum<T>;
         INSMOS_LAUNCH(sum, dim3((p.N + 15) / 16), dim3(1024), 0, s, (const float*)p.part, r.blocks, p.N, p.ld_part, (T*)db);
         HIP_TRY(hipGetLastError());
@@ -346,7 +350,9 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
             d = q.dz;
             ld_d = q.ld_dz;
         }
-        if (db) {
+        if (db && r.blocks == 1) {   // (few rows: a launch less)
+            q.db = db;
+        } else if (db) {
             q.ld_part = N;
             q.part = bump.take<float>((size_t)r.blocks * N);
             if (!q.part) return INSMOS_EWORKSPACE;
