@@ -235,7 +235,7 @@ SlopePlan slope_plan(int64_t M, int N, int dtype) {
     int64_t blocks = 2048 / r.strips;
     if (blocks < 1) blocks = 1;
     int64_t rows = ((M + blocks - 1) / blocks + step - 1) / step * step;
-    const int64_t least = 8 * step;   // (two trips of four rows in flight)
+    const int64_t least = (M <= 8 * step ? 8 : 4) * step;   // a trip has four rows in flight; two trips rather than a second workgroup and its launch
     if (rows < least) rows = least;
     if (rows > (int64_t)1 << 30) rows = (int64_t)1 << 30;
     r.rows = (int)rows;
