@@ -441,7 +441,7 @@ def main_cfg5(args, rank, world, gpu, dev, host_cores):
                    "parallelism": f"ddp{world} (per-rank batch of {B} windows; gradients all-reduced in 8 MB buckets during backward)",
                    "backend": (dist.get_backend() if world > 1 else None), "grad_buckets": (len(red.buckets) if red else 0),
                    "host_cores_per_rank": host_cores},
-        "ms_per_window": round(1000.0 * dt / (args.steps * B), 3), "timed_region_s": round(dt, 3),
+        "ms_per_window": round(1000.0 * dt / (args.steps * B), 3), "timed_region_s": round(dt, 6),
         "loss": round(loss, 4), "loss_terms": {k: round(float(v), 4) for k, v in dict(last["tb"][0] if isinstance(last["tb"], (list, tuple)) else last["tb"]).items()},
     }
     # ---- roofline of the convolution kernels of the step (forward + d/dx + d/dW, all on the fp32 MFMA path): executed flops
@@ -727,7 +727,7 @@ def main():
                               f"~{args.candidates} candidates", "parallelism": f"dp{world} (windows sharded by rank)",
                    "backend": (dist.get_backend() if (world > 1 or forced) else None)},
         "ms_per_window": round(1000.0 * dt / (args.steps * W), 3),
-        "timed_region_s": round(dt, 3),
+        "timed_region_s": round(dt, 6),
         "sustained_scans_per_sec": round(sustained, 3) if sustained is not None else None,
         # every rank's counters went through the gather: the sum holds all ranks' current points (weights are random and the
         # labels synthetic, so an IoU of these counters would mean nothing and is not printed)
