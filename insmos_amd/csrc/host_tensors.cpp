@@ -56,6 +56,7 @@ const at::Tensor& tensor_at(PyObject* list, Py_ssize_t i, const char* what, cons
     if (!THPVariable_Check(o)) throw Refused(std::string(what) + ": " + kind + " " + std::to_string(i) + " is no tensor");
     const at::Tensor& t = THPVariable_Unpack(o);
     if (t.layout() != c10::kStrided) throw Refused(std::string(what) + ": " + kind + " " + std::to_string(i) + " is sparse");
+    if (t.is_neg()) throw Refused(std::string(what) + ": " + kind + " " + std::to_string(i) + " is a negated view (resolve_neg() makes it a tensor)");
     return t;
 }
 int dtype_code(c10::ScalarType t) {
@@ -178,11 +179,11 @@ std::string shape(const at::Tensor& t) {
     return r + ")";
 }
 [[noreturn]] void refuse(const std::string& t) { throw Refused("linear: " + t); }
-const at::Tensor& arg(PyObject* o, const char* name) {
+at::Tensor arg(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) refuse(std::string(name) + " is no tensor");
     const at::Tensor& t = THPVariable_Unpack(o);
     if (t.layout() != c10::kStrided) refuse(std::string(name) + " is sparse");
-    return t;
+    return t.is_neg() ? t.resolve_neg() : t;   // (a view whose memory holds the values with the other sign)
 }
 constexpr int64_t kMost = 1 << 20;   // widths and pitches
 // t as rows of `cols` whose values are contiguous and that do not overlap (shared: they may be one row), and their pitch; a copy only where t
@@ -229,6 +230,8 @@ PyObject* guarded(F f) {   // no C++ exception leaves the module
         PyErr_SetString(PyExc_ValueError, e.what());
     } catch (const LibraryError& e) {
         raise("insmos_amd._lib", "InsmosHipError", e.what());
+    } catch (python_error& e) {   // (a hook on saved tensors that raised: checkpoints stop their recomputation that way)
+        e.restore();
     } catch (const c10::OutOfMemoryError& e) {
         raise("torch", "OutOfMemoryError", e.what_without_backtrace());   // as torch's own allocations do
     } catch (const std::exception& e) {
@@ -362,11 +365,12 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
             // an input that is not there has no edge
             const bool need_b = meta & kBias && ctx->needs_input_grad(2), need_r = meta & kResidual && ctx->needs_input_grad(meta & kBias ? 3 : 2);
             const bool z = need_r && meta & kFirst && kind != INSMOS_SLOPE_NONE;
-            const Grads g = backward_of(dys[0], saved[2], saved[0], saved[1], kind, ctx->needs_input_grad(0), ctx->needs_input_grad(1), need_b, z);
+            const at::Tensor dy = dys[0].resolve_neg();
+            const Grads g = backward_of(dy, saved[2], saved[0], saved[1], kind, ctx->needs_input_grad(0), ctx->needs_input_grad(1), need_b, z);
             out[0] = g.x;
             out[1] = g.w;
             out[2] = g.b;
-            if (need_r) out[3] = z ? g.z : dys[0];
+            if (need_r) out[3] = z ? g.z : dy;
         } catch (const LibraryError& e) {   // the tape hands a Python error on as it is
             PyGILState_STATE gil = PyGILState_Ensure();
             raise("insmos_amd._lib", "InsmosHipError", e.what());

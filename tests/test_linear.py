@@ -408,3 +408,40 @@ def test_linear_large_tiles(M, K, N, dtype):
     """Sizes that take the 256 x 256 tile (whole and with k in parts), the 128 x 128 one and 64 and 32 rows of it, each with partial last tiles."""
     for layout in ("in_out", "out_in"):
         _check(*_case(M, K, N, dtype, "gelu_tanh", True, layout, seed=8), "gelu_tanh", False)
+
+
+@pytest.mark.gpu
+def test_linear_negated_views():
+    """The imaginary part of a conjugate: a view whose memory holds the values with the other sign, as every operand and as the gradient."""
+    gen = torch.Generator().manual_seed(12)
+    imag = lambda *s: torch.conj(torch.randn(*s, dtype=torch.complex64, generator=gen).cuda()).imag   # noqa: E731
+    x, w, b, r, dy = imag(20, 12), imag(12, 9), imag(9), imag(20, 9), imag(20, 9)
+    assert x.is_neg()
+    plain = [t.resolve_neg().contiguous() for t in (x, w, b, r, dy)]
+    ins, ref = [t.detach().requires_grad_(True) for t in (x, w, b, r)], [t.requires_grad_(True) for t in plain[:4]]
+    y, want = linear(*ins, activation="silu"), linear(*ref, activation="silu")
+    assert torch.equal(y, want)
+    for g, e in zip(torch.autograd.grad(y, ins, dy), torch.autograd.grad(want, ref, plain[4])):
+        assert torch.equal(g, e)
+
+
+@pytest.mark.gpu
+def test_linear_in_checkpoints_and_with_saved_tensor_hooks():
+    """Recomputation in the backward pass and packed saved tensors give the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    gen = torch.Generator().manual_seed(13)
+    x, w, b = (torch.randn(s, generator=gen).cuda().requires_grad_(True) for s in ((50, 24), (24, 16), (16,)))
+    f = lambda x_, w_, b_: linear(x_, w_, b_, activation="gelu")   # noqa: E731
+    want = torch.autograd.grad(f(x, w, b).square().sum(), (x, w, b))
+    got = torch.autograd.grad(checkpoint(f, x, w, b, use_reentrant=False).square().sum(), (x, w, b))
+    assert all(torch.equal(g, e) for g, e in zip(got, want))
+    with torch.autograd.graph.save_on_cpu():
+        y = f(x, w, b)
+    got = torch.autograd.grad(y.square().sum(), (x, w, b))
+    assert all(torch.equal(g, e) for g, e in zip(got, want))
+    x2 = x.detach().clone().requires_grad_(True)
+    y = f(x2, w, b)
+    with torch.no_grad():
+        x2.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        torch.autograd.grad(y.sum(), w)

@@ -641,3 +641,17 @@ def test_optimizer_copies_and_pickles(bits):
         assert all(torch.equal(a, b) for a, b in zip(go(c, range(2, 4)), want))
         for p, q in zip(c.param_groups[0]["params"], ps):
             assert all(torch.equal(c.state[p][k].float(), o.state[q][k].float()) for k in o.state[q])
+
+
+@pytest.mark.gpu
+def test_negated_views_are_refused_and_inference_tensors_taken():
+    neg = torch.conj(torch.ones(300, dtype=torch.complex64, device="cuda")).imag
+    m, v, step = torch.zeros(512, device="cuda"), torch.zeros(512, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert neg.is_neg()
+    with pytest.raises(ValueError, match="negated"):
+        adamw_step([torch.ones(300, device="cuda")], [neg], m, v, step, lr=0.1)
+    with torch.inference_mode():
+        p = torch.ones(300, device="cuda")
+    assert step.item() == 0 and not bool(m.any())
+    adamw_step([p], [torch.ones(300, device="cuda")], m, v, step, lr=0.25, weight_decay=0.0, eps=0.0)   # (m / sqrt(v) = 1 in the first step)
+    assert step.item() == 1 and bool(((p - 0.75).abs() < 1e-6).all())
