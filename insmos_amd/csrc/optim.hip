@@ -67,15 +67,19 @@ __device__ __forceinline__ uint32_t mix32(uint32_t x) {
     x ^= x >> 15; x *= 0x846CA68Bu;
     return x ^ (x >> 16);
 }
-// the tensor a workgroup works on (the argument arrays are read through scalar loads: the index is the same for all lanes)
+// The tensor a workgroup works on: how many of the list's starts are not behind it.  Every lane looks at a few of them at once (a search, whose
+// reads wait for each other, cost 0.6 to 1 us more per launch: 250 tensors' norm 9.5 -> 8.6 us, 140 tensors' update 21.3 -> 20.3).
 template <class List>
 __device__ __forceinline__ int tensor_of(const List& L, uint32_t b) {
-    int lo = 0, hi = L.count;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (L.first[mid] <= b) lo = mid; else hi = mid;
+    const int lane = threadIdx.x & 63;
+    int t = -1;
+#pragma unroll
+    for (int i = 0; i < List::MOST; i += 64) {
+        const bool in = i + lane < L.count;
+        const uint32_t first = L.first[min(i + lane, List::MOST)];
+        t += __builtin_popcountll(__ballot(in && first <= b));
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(t);
 }
 // V (4 or 8) elements of a tensor from element i on; zeros past its end; `wide` = the tensor's address allows one access
 template <int V, class T>
