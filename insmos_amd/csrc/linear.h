@@ -616,18 +616,23 @@ struct Few {   // 16 bit: a chunk is 64 k, four steps of 16
     }
 };
 template <int LB>
-struct Few<float, LB> {   // fp32: a chunk is 32 k, four steps of 8 (their k in the order of Frag<float>)
+struct Few<float, LB> {   // fp32: a chunk is 32 k, four steps of 8: the lower half of the lanes has the first four of them, in 16-byte loads
     static constexpr int CHUNK = 32, TURN = 0;
     typedef f32x4 type;
     static __device__ __forceinline__ void load_x(const float* row, int k0, int K, int lane, f32x4 (&f)[4]) {
+        typedef float M4 __attribute__((ext_vector_type(4), aligned(4)));
+        if (k0 + CHUNK <= K) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            constexpr int K4[4] = {0, 4, 1, 5};
+            for (int s = 0; s < 4; ++s) f[s] = *(const M4*)(row + k0 + 8 * s + 4 * (lane >> 5));
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int k = k0 + 8 * s + 2 * (lane >> 5) + K4[e];
-                const float v = row[min(k, K - 1)];
-                f[s][e] = k < K ? v : 0.f;
+            for (int s = 0; s < 4; ++s) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int k = k0 + 8 * s + 4 * (lane >> 5) + e;
+                    const float v = row[min(k, K - 1)];
+                    f[s][e] = k < K ? v : 0.f;
+                }
             }
         }
     }
@@ -636,10 +641,9 @@ struct Few<float, LB> {   // fp32: a chunk is 32 k, four steps of 8 (their k in 
         if (LB == KC) return load_x(w + n * ld, k0, K, lane, f);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            constexpr int K4[4] = {0, 4, 1, 5};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int k = k0 + 8 * s + 2 * (lane >> 5) + K4[e];
+                const int k = k0 + 8 * s + 4 * (lane >> 5) + e;
                 const float v = w[min(k, K - 1) * ld + n];
                 f[s][e] = k < K ? v : 0.f;
             }

@@ -4,6 +4,7 @@
 //
 // The three products are linear.h's; here is what surrounds them: the choice of tile and of parts of k, the layout of operands that the
 // 16-byte loads cannot take as they are, dz with the column sums (one pass over dy and z), and the argument checks.
+#include <cmath>
 #include "linear.h"
 
 namespace insmos {
@@ -59,16 +60,27 @@ int operand(const void* p, int64_t ld, int64_t rows, int cols, int lay, int dtyp
 
 // ---- tile and parts ---------------------------------------------------------------------------------------------------------
 struct Plan { int tile, splits; };
-// Up to 32 rows (x W alone) there is a kernel of its own.  Otherwise the tile and the number of parts of k with the shortest predicted time:
+// Up to 32 rows (x W alone) there is a kernel of its own (few_rows).  Otherwise the tile and the number of parts of k with the shortest predicted time:
 //   rounds of the workgroups that fit on the chip, each k tiles x max(0.75 us, workgroups per CU x a tile's work at the CU's rate) + a fixed
 //   part for its first loads and its epilogue; with parts, their bytes at 4 TB/s and another launch.
 // Rates (all CUs together, TFLOP/s) and fixed parts (us) are measured; predicted / measured, us, bf16: 8192 x 1024 x 1024 128x128 24 / 26,
 // 256x256 39 / 33; 2048^3 128x64 29 / 32, 128x128 32 / 35; 512 x 4096 x 512 128x64 in 8 parts 18 / 15, 128x128 in 16 23 / 21; fp32:
 // 300000 x 128 x 256 128x128 234 / 231, 128x64 212 / 213; 119817 x 64 x 128 128x128 31 / 37, 128x32 29 / 33.
-Plan plan_for(int M, int N, int K, int dtype, bool xw) {   // xw: the first operand has contiguous k
+//
+// The kernel for few rows or tiles and parts, by predicted times again (us): a workgroup per 32 columns walks all of k, 8 waves taking 128 bytes
+// of it in turn, against 13 for two launches or the weights' stream; odd operands, which only the tiles need copied, add that.  Few / tiles, us:
+// bf16 1 x 4096 x 4096 12.6 / 13.9, 32 rows 17.8 / 16.4, 8 x 14336 x 4096 38 / 23.5, 4 x 8192 x 8192 26 / 28; fp32 8 x 1024 x 1024 10.8 / 13.5,
+// 8 x 2048 x 2048 17.4 / 13.3, 4 x 4096 x 8192 33.5 / 30.
+bool few_rows(int M, int N, int K, int dtype, bool odd) {
+    if (M > 32) return false;
+    const int trips = (int)((K * (int64_t)size_of(dtype) + 1023) / 1024), rounds = (N + 8191) / 8192;
+    const double few = 4 + trips * rounds * (dtype == INSMOS_F32 ? 1.7 : 1.1 + 0.0125 * M), bytes = (double)K * N * size_of(dtype);
+    return few < fmax(13, 6 + bytes / 6.5e6) + (odd ? 6 + bytes / 2.5e6 : 0);
+}
+// xw: the first operand has contiguous k; odd: an operand would have to be copied for the tiles
+Plan plan_for(int M, int N, int K, int dtype, bool xw, bool odd = false) {
     const int bk = 128 / (int)size_of(dtype), nk = (K + bk - 1) / bk;
-    // (one workgroup per 32 columns walks all of k: 16 x 8192 x 256 takes 25 us that way and 10 in parts)
-    if (M <= 32 && xw && (K <= 4096 || N >= 4096)) return {FEW, 1};
+    if (xw && few_rows(M, N, K, dtype, odd)) return {FEW, 1};
     struct Shape { int tile, bm, bn, slots; double rate, rate32, fixed; };
     static const Shape shapes[] = {{T256, 256, 256, 256, 1250, 0, 12},     {T128, 128, 128, 512, 1050, 140, 8},    {T128X64, 128, 64, 768, 800, 135, 5},
                                    {T64X128, 64, 128, 768, 800, 135, 5},  {T128X32, 128, 32, 1024, 500, 120, 3}, {T32X128, 32, 128, 1024, 500, 120, 3}};
@@ -99,8 +111,7 @@ Plan plan_for(int M, int N, int K, int dtype, bool xw) {   // xw: the first oper
     return best;
 }
 size_t plan_bytes(const Plan& r, int M, int N) { return r.splits > 1 ? pad256((size_t)r.splits * M * round_up(N, 8) * sizeof(float)) : 0; }
-int run_gemm(GemmP p, const Operand& a, const Operand& b, int dtype, Bump& ws, hipStream_t s) {
-    const Plan r = plan_for(p.M, p.N, p.K, dtype, a.lay == KC);
+int run_gemm(GemmP p, const Operand& a, const Operand& b, int dtype, const Plan& r, Bump& ws, hipStream_t s) {
     p.a = a.p; p.lda = a.ld;
     p.b = b.p; p.ldb = b.ld;
     p.splits = r.splits;
@@ -295,7 +306,9 @@ extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t
     const hipStream_t s = (hipStream_t)stream;
     Bump bump(ws, ws ? ws_bytes : 0);
     Operand a, b;
-    const bool any = plan_for((int)M, N, K, dtype, true).tile == FEW;
+    // (with FEW for odd operands less of ws is used than insmos_linear_ws_bytes counted)
+    const Plan plan = plan_for((int)M, N, K, dtype, true, !loadable(x, ld_x, dtype) || !loadable(w, ld_w, dtype));
+    const bool any = plan.tile == FEW;
     int rc = operand(x, ld_x, M, K, KC, dtype, any, bump, s, &a);
     if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, KC, dtype, any, bump, s, &b) : operand(w, ld_w, K, N, NC, dtype, any, bump, s, &b);
     if (rc != INSMOS_OK) return rc;
@@ -306,7 +319,7 @@ extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t
     p.y = y; p.ld_y = ld_y;
     p.slope = slope; p.ld_slope = ld_slope;
     p.act = act;
-    return run_gemm(p, a, b, dtype, bump, s);
+    return run_gemm(p, a, b, dtype, plan, bump, s);
 }
 
 extern "C" size_t insmos_linear_backward_ws_bytes(int64_t M, int K, int N, int dtype) {
@@ -364,14 +377,15 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
     }
     if (dx) {   // (M, K) = dz (M, N) W^T: k of this product is N
         Operand a, b;
-        const bool any = plan_for((int)M, K, N, dtype, true).tile == FEW;
+        const Plan plan = plan_for((int)M, K, N, dtype, true, !loadable(d, ld_d, dtype) || !loadable(w, ld_w, dtype));
+        const bool any = plan.tile == FEW;
         rc = operand(d, ld_d, M, N, KC, dtype, any, bump, s, &a);
         if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, NC, dtype, any, bump, s, &b) : operand(w, ld_w, K, N, KC, dtype, any, bump, s, &b);
         if (rc != INSMOS_OK) return rc;
         GemmP p = {};
         p.M = (int)M; p.N = K; p.K = N;
         p.y = dx; p.ld_y = ld_dx;
-        rc = run_gemm(p, a, b, dtype, bump, s);
+        rc = run_gemm(p, a, b, dtype, plan, bump, s);
         if (rc != INSMOS_OK) return rc;
     }
     if (dw) {   // (K, N) = x^T dz, or its transpose for a (N, K) weight: k of this product is M
@@ -382,7 +396,8 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
         GemmP p = {};
         p.M = w_out_in ? N : K; p.N = w_out_in ? K : N; p.K = (int)M;
         p.y = dw; p.ld_y = ld_dw;
-        rc = w_out_in ? run_gemm(p, b, a, dtype, bump, s) : run_gemm(p, a, b, dtype, bump, s);
+        const Plan plan = plan_for(p.M, p.N, p.K, dtype, false);
+        rc = w_out_in ? run_gemm(p, b, a, dtype, plan, bump, s) : run_gemm(p, a, b, dtype, plan, bump, s);
     }
     return rc;
 }

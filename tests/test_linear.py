@@ -445,3 +445,12 @@ def test_linear_in_checkpoints_and_with_saved_tensor_hooks():
         x2.add_(1.0)
     with pytest.raises(RuntimeError, match="modified"):
         torch.autograd.grad(y.sum(), w)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("M,K,N", [(5, 9001, 40), (32, 4096, 160), (9, 6000, 1030), (1, 600, 9000), (31, 77, 8200), (3, 1025, 512)])
+def test_linear_few_rows_both_ways(M, K, N, dtype):
+    """Up to 32 rows: sizes on either side of the choice between their own kernel and tiles with parts of k, odd operands among them."""
+    for layout in ("in_out", "out_in"):
+        _check(*_case(M, K, N, dtype, "silu", True, layout, seed=17), "silu", True)
