@@ -8,8 +8,7 @@
 Optimiser and schedule as models/models.py:188-193 (Adam(lr, weight_decay) + StepLR(step_size=LR_EPOCH, gamma=LR_DECAY)); --optimizer hip runs
 that Adam as one short chain of launches over all parameters (insmos_amd.optim.AdamW), hip8 with its moments in 8 bits;
 gradients are exchanged with insmos_amd.ddp.BucketedGradReducer (one RCCL all-reduce per 8 MB bucket) when WORLD_SIZE > 1.
-The trained tensors go back into a Lightning-shaped checkpoint that insmos_amd.models.InsMOSNet / predict_mos load.
-(Written at the end of round 1 after the GPU budget was spent: the pieces it calls are tested, this loop itself has not run.)"""
+The trained tensors go back into a Lightning-shaped checkpoint that insmos_amd.models.InsMOSNet / predict_mos load."""
 import argparse
 import os
 import sys
