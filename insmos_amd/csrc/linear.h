@@ -77,8 +77,8 @@ __device__ __forceinline__ float normal_tail(float z, float& e) {
     return p * t * e;
 }
 // act(z) in place, and act'(z), act != INSMOS_ACT_NONE: z times a weight between 0 and 1; silu's and the tanh form's are sigmoids: (1 + tanh u) / 2
-// = sigmoid(2 u).  (One formula for both: the epilogue's code is part of every tile's time when it has to be fetched.)  The choice stands outside
-// the loops: eight values' chains then run side by side (inside, 33953 x 210 x 142 bf16 with gelu took 34 us, and 18 without an activation).
+// = sigmoid(2 u).  The choice stands outside the loops: eight values' chains then run side by side (inside, 33953 x 210 x 142 bf16 with gelu took
+// 34 us, and 18 without an activation).
 __device__ __forceinline__ void activate8(f32x8& v, int act, f32x8& slope) {
     if (act == INSMOS_ACT_RELU) {
 #pragma unroll
@@ -96,25 +96,32 @@ __device__ __forceinline__ void activate8(f32x8& v, int act, f32x8& slope) {
             slope[i] = fmaf(z * 0.3989422804014327f, e, phi);
             v[i] = z * phi;
         }
-    } else {
-        const float c0 = act == INSMOS_ACT_SILU ? 1.f : 2.f * kGelu0, c1 = act == INSMOS_ACT_SILU ? 0.f : 2.f * kGelu0 * kGelu1;
-        const float d0 = -kLog2E * c0, d1 = -kLog2E * c1;
+    } else if (act == INSMOS_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float z = v[i], z2 = fminf(z * z, 3e38f);   // (c1 = 0 times inf would be none)
-            const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * fmaf(d1, z2, d0))), y = z * s;
+            const float z = v[i], s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2E * z)), y = z * s;
+            slope[i] = fmaf(-y, s, y) + s;
+            v[i] = y;
+        }
+    } else {
+        constexpr float c0 = 2.f * kGelu0, c1 = 2.f * kGelu0 * kGelu1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float z = v[i], z2 = fminf(z * z, 3e38f);   // (its slope has 0 times the square far out)
+            const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * fmaf(-kLog2E * c1, z2, -kLog2E * c0))), y = z * s;
             slope[i] = fmaf(fmaf(-y, s, y), fmaf(3.f * c1, z2, c0), s);
             v[i] = y;
         }
     }
 }
 // What the backward pass is given of act'(z): the value itself in fp32; with 16-bit types 16 bits of it in steps of 2^-15 from -1/2 on (all
-// slopes lie in -0.13 .. 1.13), 0xFFFF where it is none.  A z rounded to the type would cost the same bytes and ten times the error (fp16), and
-// the backward would have to compute the slope again.
+// slopes lie in -0.13 .. 1.13, so codes in 12 000 .. 53 500), 0 where it is none.  In two instructions, the first clamped to 0 .. 1 (which makes a
+// NaN 0): added to 2^23, a value is rounded to a whole number that lies in the sum's lowest bits.  A z rounded to the type would cost the same
+// bytes and ten times the error (fp16), and the backward would have to compute the slope again.
 template <class T> struct Slope {
     typedef uint16_t t;
-    static __device__ __forceinline__ uint16_t store(float s) { return s == s ? (uint16_t)(int)rintf(fminf(fmaxf(s + 0.5f, 0.f), 1.99f) * 32768.f) : (uint16_t)0xFFFF; }
-    static __device__ __forceinline__ float load(uint16_t c) { return c == 0xFFFF ? __builtin_nanf("") : (float)c * 0x1p-15f - 0.5f; }
+    static __device__ __forceinline__ uint16_t store(float s) { return (uint16_t)__float_as_uint(fmaf(fminf(fmaxf(fmaf(s, 0.5f, 0.25f), 0.f), 1.f), 0x1p16f, 0x1p23f)); }
+    static __device__ __forceinline__ float load(uint16_t c) { return c == 0 ? __builtin_nanf("") : (float)c * 0x1p-15f - 0.5f; }
 };
 template <> struct Slope<float> {
     typedef float t;

@@ -454,3 +454,24 @@ def test_linear_few_rows_both_ways(M, K, N, dtype):
     """Up to 32 rows: sizes on either side of the choice between their own kernel and tiles with parts of k, odd operands among them."""
     for layout in ("in_out", "out_in"):
         _check(*_case(M, K, N, dtype, "silu", True, layout, seed=17), "silu", True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,bits", [("bf16", (0x7FC0, 0x7FFF, 0x7F81, -0x40, -1)), ("fp16", (0x7E00, 0x7FFF, 0x7C01, 0x7D55, -1))])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_linear_nan_of_any_payload_reaches_the_gradients(dtype, bits, act):
+    """NaNs with all kinds of bits in x, in the bias and in the residual: the slopes that are stored in 16 bits say so too (dz, and with it dx and the
+    weight's gradient, is NaN where z is)."""
+    t = DTYPES[dtype]
+    x = torch.ones(len(bits) + 40, 16, dtype=t, device="cuda")
+    x[:len(bits), 0] = torch.tensor(bits, dtype=torch.int16).view(t).cuda()
+    w, r = torch.full((16, 24), 0.1, dtype=t, device="cuda"), torch.zeros(len(bits) + 40, 24, dtype=t, device="cuda")
+    r[-1, 3] = torch.tensor(bits[1], dtype=torch.int16).view(t).cuda()
+    ins = [v.requires_grad_(True) for v in (x, w, r)]
+    y = linear(x, w, None, r, activation=act, residual_first=True)
+    dx, dw, dr = torch.autograd.grad(y, ins, torch.ones_like(y))
+    want = torch.zeros_like(y, dtype=torch.bool)
+    want[:len(bits)] = True
+    want[-1, 3] = True
+    assert torch.equal(y.isnan(), want) and torch.equal(dr.isnan(), want)
+    assert torch.equal(dx.isnan().any(1), want.any(1)) and bool(dw.isnan().all())
