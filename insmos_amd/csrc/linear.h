@@ -456,7 +456,7 @@ struct Gemm {
 
 // Workgroup w runs on XCD w % 8 (each has an L2 of its own), so every XCD gets a contiguous run of items, walked in groups of 8 tile rows: the
 // operands of the tiles in flight on one XCD stay in its L2 (groups of 4, 8 or 16: within 3 %).  Bound by the matrix units from a K of some hundreds
-// on: 8192 x 4096 x 8192 bf16 with gelu_tanh and a residual 486 us = 1131 TFLOP/s (the platform's plain product: 1186), 4096^3 fp32 982 us = 140 of
+// on: 8192 x 4096 x 8192 bf16 with gelu_tanh and a residual 486 .. 496 us = 1110 .. 1131 TFLOP/s (the platform's plain product: 1186), 4096^3 fp32 982 us = 140 of
 // 157; below that by the epilogue's lines and vector work (some 12 us per 256 x 256 tile, 8 for two of 128 x 128 side by side).
 template <class T, int LA, int LB, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_gemm(const GemmP p) {
