@@ -511,7 +511,7 @@ def linear(x, weight, bias=None, residual=None, activation=None, residual_first=
     x (..., cin): rows of any pitch; weight (cin, cout), one tap of sparse_conv(); an nn.Linear weight's transpose (a (cout, cin) tensor's
     .t()) is read as it lies.  bias (cout,).  residual: the output's shape (an expanded one works: rows of pitch 0).  activation: None,
     "relu", "gelu" (erf), "gelu_tanh" or "silu".  All tensors of one dtype -- float32, bfloat16 or float16 -- on one GPU; sums in fp32.
-    Widths up to 2^20.  Differentiable once in all four tensors; without gradients nothing is kept for a backward pass.  In 16 bits the
+    Widths up to 2^20.  Differentiable once in all four tensors, backwards (a forward-mode tangent is refused); without gradients nothing is kept for a backward pass.  In 16 bits the
     backward rounds dz once, for the products.  Forward and backward can be captured into a graph; the backward refuses where a graph that
     was recorded on the default stream shares its inputs and is still alive."""
     try:

@@ -30,6 +30,7 @@ struct Refused : std::exception {
     explicit Refused(std::string t) : text(std::move(t)) {}
     const char* what() const noexcept override { return text.c_str(); }
 };
+struct Unsupported : Refused { using Refused::Refused; };   // NotImplementedError
 
 // whether a tensor fills its memory without gaps or overlaps, in some order of its dimensions
 bool dense(const at::Tensor& t) {
@@ -183,6 +184,7 @@ at::Tensor arg(PyObject* o, const char* name) {
     if (!THPVariable_Check(o)) refuse(std::string(name) + " is no tensor");
     const at::Tensor& t = THPVariable_Unpack(o);
     if (t.layout() != c10::kStrided) refuse(std::string(name) + " is sparse");
+    if (t._fw_grad(0).defined()) throw Unsupported(std::string("linear: ") + name + " has a forward-mode tangent, and linear has no forward-mode derivative");
     return t.is_neg() ? t.resolve_neg() : t;   // (a view whose memory holds the values with the other sign)
 }
 constexpr int64_t kMost = 1 << 20;   // widths and pitches
@@ -226,6 +228,8 @@ template <class F>
 PyObject* guarded(F f) {   // no C++ exception leaves the module
     try {
         return f();
+    } catch (const Unsupported& e) {
+        PyErr_SetString(PyExc_NotImplementedError, e.what());
     } catch (const Refused& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
     } catch (const LibraryError& e) {
