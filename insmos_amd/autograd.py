@@ -17,8 +17,10 @@ import contextlib
 import ctypes
 import os
 import threading
+from typing import List, Optional, Tuple
 
 import torch
+from torch.overrides import handle_torch_function, has_torch_function_variadic
 
 from . import _lib
 from .engine import _padc
@@ -511,14 +513,75 @@ def linear(x, weight, bias=None, residual=None, activation=None, residual_first=
     x (..., cin): rows of any pitch; weight (cin, cout), one tap of sparse_conv(); an nn.Linear weight's transpose (a (cout, cin) tensor's
     .t()) is read as it lies.  bias (cout,).  residual: the output's shape (an expanded one works: rows of pitch 0).  activation: None,
     "relu", "gelu" (erf), "gelu_tanh" or "silu".  All tensors of one dtype -- float32, bfloat16 or float16 -- on one GPU; sums in fp32.
-    Widths up to 2^20.  Differentiable once in all four tensors, backwards (a forward-mode tangent is refused); without gradients nothing is kept for a backward pass.  In 16 bits the
-    backward rounds dz once, for the products.  Forward and backward can be captured into a graph; the backward refuses where a graph that
-    was recorded on the default stream shares its inputs and is still alive."""
+    Widths up to 2^20.  Differentiable once in all four tensors, backwards (a forward-mode tangent is refused, and so are torch.func's
+    transforms); without gradients nothing is kept for a backward pass.  Tracers, fake tensors and dispatch modes see it as insmos::linear.
+    In 16 bits the backward rounds dz once, for the products.  Forward and backward can be captured into a graph; the backward refuses where
+    a graph that was recorded on the default stream shares its inputs and is still alive."""
     try:
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):
         raise ValueError(f"linear: activation is one of {list(_ACTIVATIONS)}, not {activation!r}") from None
-    return _host().linear(x, weight, bias, residual, act, residual_first)
+    if has_torch_function_variadic(x, weight, bias, residual):     # (subclasses that say themselves what becomes of a function's results)
+        return handle_torch_function(linear, (x, weight, bias, residual), x, weight, bias, residual, activation, residual_first)
+    y = _host().linear(x, weight, bias, residual, act, residual_first)
+    return torch.ops.insmos.linear(x, weight, bias, residual, act, bool(residual_first))[0] if y is NotImplemented else y
+
+
+# The layer as a registered operator, insmos::linear, which tracers (torch.jit.trace, make_fx), fake tensors and dispatch modes see: (y, slopes).
+# linear() takes it only where one of those is there: a registered Python operator costs some 30 us more per call.
+@torch.library.custom_op("insmos::linear", mutates_args=())
+def _linear_op(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor], activation: int,
+               residual_first: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    y, slope = _host().linear_forward(x, weight, bias, residual, activation, residual_first)
+    return y, x.new_empty(0) if slope is None else slope
+
+
+@torch.library.custom_op("insmos::linear_backward", mutates_args=())
+def _linear_backward_op(dy: torch.Tensor, slope: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, activation: int, residual_behind: bool,
+                        needs: List[bool]) -> List[torch.Tensor]:
+    grads = _host().linear_backward(dy, slope, x, weight, activation, residual_behind, *needs)
+    return [x.new_empty(0) if g is None else g for g in (*grads[:3], None if grads[3] is None else grads[3].contiguous())]
+
+
+def _slopes_of(activation, residual_behind):
+    """Whether the backward pass takes stored slopes (relu: y itself, unless a residual was added behind it)."""
+    return activation > 1 or (activation == 1 and residual_behind)
+
+
+@_linear_op.register_fake
+def _(x, weight, bias, residual, activation, residual_first):
+    y = x.new_empty((*x.shape[:-1], weight.shape[1]))
+    if not _slopes_of(activation, residual is not None and not residual_first):
+        return y, x.new_empty(0)
+    chunk = 16 // x.element_size()
+    rows = x.numel() // x.shape[-1]
+    return y, x.new_empty((rows, (weight.shape[1] + chunk - 1) // chunk * chunk), dtype=torch.float32 if x.dtype == torch.float32 else torch.int16)
+
+
+@_linear_backward_op.register_fake
+def _(dy, slope, x, weight, activation, residual_behind, needs):
+    shapes = (x.shape, weight.shape, weight.shape[1:], dy.shape)
+    grads = [x.new_empty(s if n else 0) for s, n in zip(shapes, needs)]
+    if needs[1] and weight.stride(1) != 1 and weight.stride(0) == 1:     # (the weight's own layout)
+        grads[1] = x.new_empty(weight.shape[::-1]).t()
+    return grads
+
+
+def _linear_op_setup(ctx, inputs, output):
+    x, weight, bias, residual, activation, residual_first = inputs
+    ctx.activation, ctx.first, ctx.behind = activation, residual_first, residual is not None and not residual_first
+    ctx.save_for_backward(x, weight, output[1] if _slopes_of(activation, ctx.behind) else output[0])
+
+
+def _linear_op_backward(ctx, dy, _):
+    x, weight, slope = ctx.saved_tensors
+    nx, nw, nb, nr = ctx.needs_input_grad[:4]
+    nz = nr and ctx.first and ctx.activation != 0
+    dx, dw, db, dz = torch.ops.insmos.linear_backward(dy, slope, x, weight, ctx.activation, ctx.behind, [nx, nw, nb, nz])
+    return dx if nx else None, dw if nw else None, db if nb else None, (dz if nz else dy) if nr else None, None, None
+
+
+_linear_op.register_autograd(_linear_op_backward, setup_context=_linear_op_setup)
 
 
 # ---------------------------------------------------------------------------------------------------------------------

@@ -3,10 +3,13 @@
 //   opt_table: one pass over the optimiser step's lists that checks them and writes the InsmosOptTensor table (include/insmos_hip.h).  From
 //     Python the same pass costs ten attribute reads per tensor (some 0.1 us each: 0.5 ms for 250 tensors, ten times what the GPU needs).
 //   linear: the layer with its node on the autograd tape -- checks, allocations and the calls of insmos_linear(_backward) (20 us forward and
-//     90 with a backward from Python, where the GPU needs 7 for one row).
+//     90 with a backward from Python, where the GPU needs 7 for one row).  linear_forward, linear_backward: the same without a node, for the
+//     registered operator that linear() takes where a program is being traced.
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -187,6 +190,16 @@ at::Tensor arg(PyObject* o, const char* name) {
     if (t._fw_grad(0).defined()) throw Unsupported(std::string("linear: ") + name + " has a forward-mode tangent, and linear has no forward-mode derivative");
     return t.is_neg() ? t.resolve_neg() : t;   // (a view whose memory holds the values with the other sign)
 }
+// Whether something outside takes down which operators run (a tracer, a dispatch mode) or a tensor stands for another one (a fake one, a wrapper):
+// the calls below would pass it by.
+bool observed(std::initializer_list<const at::Tensor*> tensors) {
+    if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
+        throw Unsupported("linear: no rules for torch.func's transforms (grad, vmap, jvp)");
+    if (at::tracer::impl::is_dispatch_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set()) return true;
+    for (const at::Tensor* t : tensors)
+        if (t->defined() && (t->is_meta() || t->key_set().has(c10::DispatchKey::Python) || t->key_set().has(c10::DispatchKey::Functionalize))) return true;
+    return false;
+}
 constexpr int64_t kMost = 1 << 20;   // widths and pitches
 // t as rows of `cols` whose values are contiguous and that do not overlap (shared: they may be one row), and their pitch; a copy only where t
 // is not so
@@ -249,6 +262,11 @@ PyObject* guarded(F f) {   // no C++ exception leaves the module
 int64_t padded(int64_t cols, const at::Tensor& like) {
     const int64_t chunk = 16 / (int64_t)like.element_size();
     return (cols + chunk - 1) / chunk * chunk;
+}
+
+// What the backward pass is given of the activation.  relu: y > 0 says what z > 0 does, unless a residual was added behind it.
+int slope_kind(int act, bool residual, bool first) {
+    return act == INSMOS_ACT_NONE ? INSMOS_SLOPE_NONE : act == INSMOS_ACT_RELU && (!residual || first) ? INSMOS_SLOPE_SIGN : INSMOS_SLOPE_STORED;
 }
 
 struct Layer { at::Tensor x, w, b, r; int act; bool first; };   // b, r: undefined where there is none
@@ -349,12 +367,10 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     using Maybe = std::optional<at::Tensor>;
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const Maybe& b, const Maybe& r, int64_t act,
                               bool first) {
-        // relu: y > 0 says what z > 0 does, unless a residual was added behind it
-        const bool of_y = act == INSMOS_ACT_RELU && (!r || first);
-        const auto out = forward_of({x, w, b.value_or(at::Tensor()), r.value_or(at::Tensor()), (int)act, first}, act != INSMOS_ACT_NONE && !of_y);
-        ctx->save_for_backward({x, w, of_y ? out.first : out.second});
-        ctx->saved_data["meta"] = (act == INSMOS_ACT_NONE ? INSMOS_SLOPE_NONE : of_y ? INSMOS_SLOPE_SIGN : INSMOS_SLOPE_STORED) + (first ? kFirst : 0) +
-                                  (b ? kBias : 0) + (r ? kResidual : 0);
+        const int kind = slope_kind((int)act, r.has_value(), first);
+        const auto out = forward_of({x, w, b.value_or(at::Tensor()), r.value_or(at::Tensor()), (int)act, first}, kind == INSMOS_SLOPE_STORED);
+        ctx->save_for_backward({x, w, kind == INSMOS_SLOPE_SIGN ? out.first : out.second});
+        ctx->saved_data["meta"] = kind + (first ? kFirst : 0) + (b ? kBias : 0) + (r ? kResidual : 0);
         return out.first;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dys) {
@@ -392,12 +408,39 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
         return out;
     }
 };
-// linear(x, weight, bias or None, residual or None, act, residual_first) -> y
+Layer layer_of(PyObject* const* a) {
+    return {arg(a[0], "x"), arg(a[1], "weight"), a[2] == Py_None ? at::Tensor() : arg(a[2], "bias"), a[3] == Py_None ? at::Tensor() : arg(a[3], "residual"),
+            (int)PyLong_AsLong(a[4]), PyObject_IsTrue(a[5]) == 1};
+}
+// linear_forward(x, weight, bias or None, residual or None, act, residual_first) -> (y, slopes or None)
+PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 6 || !g_linear) refuse("internal call");
+        const Layer l = layer_of(a);
+        const auto out = forward_of(l, slope_kind(l.act, l.r.defined(), l.first) == INSMOS_SLOPE_STORED);
+        return Py_BuildValue("NN", wrap(out.first), wrap(out.second));
+    });
+}
+// linear_backward(dy, slopes or y or None, x, weight, act, residual behind the activation, need_x, need_w, need_b, need_z) -> (dx, dw, db, dz), None
+// where not needed
+PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 10 || !g_linear) refuse("internal call");
+        refuse_default_stream();
+        bool is[5];
+        for (int i = 0; i < 5; ++i) is[i] = PyObject_IsTrue(a[5 + i]) == 1;
+        const int kind = slope_kind((int)PyLong_AsLong(a[4]), is[0], !is[0]);
+        const Grads g = backward_of(arg(a[0], "the gradient"), a[1] == Py_None ? at::Tensor() : arg(a[1], "slope"), arg(a[2], "x"), arg(a[3], "weight"),
+                                    kind, is[1], is[2], is[3], is[4]);
+        return Py_BuildValue("NNNN", wrap(g.x), wrap(g.w), wrap(g.b), wrap(g.z));
+    });
+}
+// linear(x, weight, bias or None, residual or None, act, residual_first) -> y, or NotImplemented where the registered operator has to be called
 PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         if (n_args != 6 || !g_linear) refuse("internal call");
-        Layer l{arg(a[0], "x"), arg(a[1], "weight"), a[2] == Py_None ? at::Tensor() : arg(a[2], "bias"), a[3] == Py_None ? at::Tensor() : arg(a[3], "residual"),
-                (int)PyLong_AsLong(a[4]), PyObject_IsTrue(a[5]) == 1};
+        const Layer l = layer_of(a);
+        if (observed({&l.x, &l.w, &l.b, &l.r})) Py_RETURN_NOTIMPLEMENTED;
         bool tape = false;
         if (at::GradMode::is_enabled())
             for (const at::Tensor* t : {&l.x, &l.w, &l.b, &l.r}) tape = tape || (t->defined() && t->requires_grad());
@@ -413,6 +456,8 @@ PyMethodDef kMethods[] = {{"opt_order", opt_order, METH_O, "a hash of sizes and 
                           {"opt_table", opt_table, METH_VARARGS, "checks lists of tensors and writes their InsmosOptTensor table"},
                           {"bind_linear", bind_linear, METH_VARARGS, "addresses of the library's functions"},
                           {"linear", (PyCFunction)(void (*)())linear, METH_FASTCALL, "the layer, on the autograd tape"},
+                          {"linear_forward", (PyCFunction)(void (*)())linear_forward, METH_FASTCALL, "the layer and its slopes"},
+                          {"linear_backward", (PyCFunction)(void (*)())linear_backward, METH_FASTCALL, "its gradients"},
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 }  // namespace
