@@ -857,7 +857,8 @@ int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dt
  * (steps of 2^-15 from -1/2; 0: not a number), 16-byte aligned, ld_slope a multiple of 16 bytes that holds N rounded up to 16 bytes; not
  * without an activation.
  * Backward: dz = dy act'(z);  dx = dz W^T;  dw = x^T dz in the weight's layout;  db = column sums of dz (before its rounding to the type).
- * slope_kind: INSMOS_SLOPE_NONE (no activation), INSMOS_SLOPE_SIGN (slope holds y = relu(z), of which the sign counts) or INSMOS_SLOPE_STORED.
+ * slope_kind: INSMOS_SLOPE_NONE (no activation), INSMOS_SLOPE_SIGN (slope holds y = relu(z), of which the sign counts), INSMOS_SLOPE_STORED
+ * (dy times the stored slope, whatever dy is) or INSMOS_SLOPE_GATE (a relu's stored slopes, 0 or 1: where it is shut dz is 0, whatever dy is).
  * Each of dx, dw, db, dz may be NULL; dz: 16-byte aligned rows like slope's.
  * ws: 16-byte aligned, insmos_linear*_ws_bytes bytes.  M = 0 is no work for insmos_linear and refused by the backward.  Outputs overlap
  * neither inputs nor each other.
@@ -870,6 +871,7 @@ int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dt
 #define INSMOS_SLOPE_NONE 0
 #define INSMOS_SLOPE_SIGN 1
 #define INSMOS_SLOPE_STORED 2
+#define INSMOS_SLOPE_GATE 3
 size_t insmos_linear_ws_bytes(int64_t M, int K, int N, int dtype);
 int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, const void* bias, const void* residual,
                   int64_t ld_res, int residual_first, int act, int64_t M, int K, int N, int dtype, void* y, int64_t ld_y,

@@ -264,9 +264,11 @@ int64_t padded(int64_t cols, const at::Tensor& like) {
     return (cols + chunk - 1) / chunk * chunk;
 }
 
-// What the backward pass is given of the activation.  relu: y > 0 says what z > 0 does, unless a residual was added behind it.
+// What the backward pass is given of the activation.  relu: y > 0 says what z > 0 does, unless a residual was added behind it.  (y as rounded: a z
+// below fp16's smallest number counts as shut, as it does to a relu of a rounded product.)
 int slope_kind(int act, bool residual, bool first) {
-    return act == INSMOS_ACT_NONE ? INSMOS_SLOPE_NONE : act == INSMOS_ACT_RELU && (!residual || first) ? INSMOS_SLOPE_SIGN : INSMOS_SLOPE_STORED;
+    if (act == INSMOS_ACT_NONE) return INSMOS_SLOPE_NONE;
+    return act != INSMOS_ACT_RELU ? INSMOS_SLOPE_STORED : residual && !first ? INSMOS_SLOPE_GATE : INSMOS_SLOPE_SIGN;
 }
 
 struct Layer { at::Tensor x, w, b, r; int act; bool first; };   // b, r: undefined where there is none
@@ -337,7 +339,7 @@ Grads backward_of(const at::Tensor& dy, const at::Tensor& slope, const at::Tenso
             const Rows d = rows_of(dy, cout), xr = rows_of(x, cin);
             const size_t need = g_backward_ws(n, (int)cin, (int)cout, dt);
             const at::Tensor ws = at::empty({(int64_t)need}, opt.dtype(at::kByte));
-            checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(slope), kind == INSMOS_SLOPE_STORED ? ld : cout, kind, xr.t.data_ptr(), xr.ld, wt.t.data_ptr(),
+            checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(slope), kind >= INSMOS_SLOPE_STORED ? ld : cout, kind, xr.t.data_ptr(), xr.ld, wt.t.data_ptr(),
                                wt.ld, wt.out_in, n, (int)cin, (int)cout, dt, at_ptr(g.x), cin, at_ptr(g.w), wt.out_in ? cin : cout, at_ptr(g.b),
                                at_ptr(g.z), ld, ws.data_ptr(), need, stream_of(x)), "insmos_linear_backward");
         }
@@ -361,14 +363,14 @@ void refuse_default_stream() {
             refuse("a backward pass is being captured, but a graph on the default stream shares its inputs and is alive (drop that graph's outputs before the capture)");
     }
 }
-// The node keeps x, W and the activation's slopes (16 bits each with 16-bit types; y itself for relu, whose slope is its sign).
+// The node keeps x, W and the activation's slopes (16 bits each with 16-bit types; y itself for a relu without a residual behind it).
 struct LinearNode : torch::autograd::Function<LinearNode> {
     enum : int64_t { kFirst = 4, kBias = 8, kResidual = 16 };   // beside the two bits of INSMOS_SLOPE_*
     using Maybe = std::optional<at::Tensor>;
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const Maybe& b, const Maybe& r, int64_t act,
                               bool first) {
         const int kind = slope_kind((int)act, r.has_value(), first);
-        const auto out = forward_of({x, w, b.value_or(at::Tensor()), r.value_or(at::Tensor()), (int)act, first}, kind == INSMOS_SLOPE_STORED);
+        const auto out = forward_of({x, w, b.value_or(at::Tensor()), r.value_or(at::Tensor()), (int)act, first}, kind >= INSMOS_SLOPE_STORED);
         ctx->save_for_backward({x, w, kind == INSMOS_SLOPE_SIGN ? out.first : out.second});
         ctx->saved_data["meta"] = kind + (first ? kFirst : 0) + (b ? kBias : 0) + (r ? kResidual : 0);
         return out.first;
@@ -417,7 +419,7 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return guarded([&]() -> PyObject* {
         if (n_args != 6 || !g_linear) refuse("internal call");
         const Layer l = layer_of(a);
-        const auto out = forward_of(l, slope_kind(l.act, l.r.defined(), l.first) == INSMOS_SLOPE_STORED);
+        const auto out = forward_of(l, slope_kind(l.act, l.r.defined(), l.first) >= INSMOS_SLOPE_STORED);
         return Py_BuildValue("NN", wrap(out.first), wrap(out.second));
     });
 }

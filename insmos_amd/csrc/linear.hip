@@ -127,7 +127,7 @@ int run_gemm(GemmP p, const Operand& a, const Operand& b, int dtype, const Plan&
 // ---- dz and the column sums -------------------------------------------------------------------------------------------------
 struct SlopeP {
     const void* dy;
-    const void* slope;   // INSMOS_SLOPE_SIGN: y; INSMOS_SLOPE_STORED: what the forward stored
+    const void* slope;   // INSMOS_SLOPE_SIGN: y; INSMOS_SLOPE_STORED, INSMOS_SLOPE_GATE: what the forward stored
     void* dz;            // or null: column sums alone
     float* part;         // [row blocks][ld_part] or null
     void* db;            // one row block: the sums' place, in the type, or null
@@ -145,6 +145,7 @@ __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {
     typedef T TV __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));   // (16 bytes at any address)
     typedef typename Slope<T>::t S;
     typedef S SV __attribute__((ext_vector_type(16 / sizeof(T))));
+    constexpr bool STORED = KIND == INSMOS_SLOPE_STORED || KIND == INSMOS_SLOPE_GATE;
     const int lanes = p.lanes, rl = 256 / lanes, cl = threadIdx.x % lanes, r0 = threadIdx.x / lanes;
     const int n = (blockIdx.x * lanes + cl) * V;
     const int64_t from = (int64_t)blockIdx.y * p.rows, to = min(p.M, from + p.rows);
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {
                 else
 #pragma unroll
                     for (int e = 0; e < V; ++e) a[u][e] = n + e < p.N ? dy[e] : (T)0.f;
-                if (KIND == INSMOS_SLOPE_STORED) c[u] = *(const SV*)((const S*)p.slope + q * p.ld_slope + n);   // (rows of whole chunks)
+                if (STORED) c[u] = *(const SV*)((const S*)p.slope + q * p.ld_slope + n);   // (rows of whole chunks)
                 if (KIND == INSMOS_SLOPE_SIGN) {
                     const T* yy = (const T*)p.slope + q * p.ld_slope + n;
                     if (whole) y[u] = *(const TV*)yy;
@@ -181,13 +182,10 @@ __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     float d = (float)a[u][e];
-                    if (KIND == INSMOS_SLOPE_STORED && n + e < p.N) {
-                        const float v = Slope<T>::load(c[u][e]);
-                        d = v == 0.f ? 0.f : d * v;   // (where a relu is shut, whatever comes from behind stays there)
-                    }
-                    if (KIND == INSMOS_SLOPE_SIGN) {
-                        const float v = (float)y[u][e];
-                        d = v > 0.f ? d : (v != v ? v : 0.f);
+                    if (KIND == INSMOS_SLOPE_STORED && n + e < p.N) d *= Slope<T>::load(c[u][e]);   // (inf and NaN stay what they are)
+                    if (KIND == INSMOS_SLOPE_SIGN || (KIND == INSMOS_SLOPE_GATE && n + e < p.N)) {
+                        const float v = KIND == INSMOS_SLOPE_SIGN ? (float)y[u][e] : Slope<T>::load(c[u][e]);
+                        d = v > 0.f ? d : (v != v ? v : 0.f);   // (where a relu is shut, whatever comes from behind stays there)
                     }
                     sum[e] += d;
                     out[e] = (T)d;
@@ -257,6 +255,7 @@ SlopePlan slope_plan(int64_t M, int N, int dtype) {
 template <class T>
 int run_slope_t(const SlopeP& p, const SlopePlan& r, void* db, hipStream_t s) {
     const auto kernel = p.kind == INSMOS_SLOPE_STORED ? k_linear_slope<T, INSMOS_SLOPE_STORED>
+                        : p.kind == INSMOS_SLOPE_GATE ? k_linear_slope<T, INSMOS_SLOPE_GATE>
                         : p.kind == INSMOS_SLOPE_SIGN ? k_linear_slope<T, INSMOS_SLOPE_SIGN> : k_linear_slope<T, INSMOS_SLOPE_NONE>;
     INSMOS_LAUNCH(kernel, dim3(r.strips, r.blocks), dim3(256), 0, s, p);
     HIP_TRY(hipGetLastError());
@@ -333,10 +332,10 @@ extern "C" size_t insmos_linear_backward_ws_bytes(int64_t M, int K, int N, int d
 extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void* slope, int64_t ld_slope, int slope_kind, const void* x,
                                       int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, int64_t M, int K, int N, int dtype, void* dx, int64_t ld_dx, void* dw,
                                       int64_t ld_dw, void* db, void* dz, int64_t ld_dz, void* ws, size_t ws_bytes, void* stream) {
-    if (!good_shape(M, K, N, dtype) || M < 1 || slope_kind < INSMOS_SLOPE_NONE || slope_kind > INSMOS_SLOPE_STORED) return INSMOS_EINVAL;
+    if (!good_shape(M, K, N, dtype) || M < 1 || slope_kind < INSMOS_SLOPE_NONE || slope_kind > INSMOS_SLOPE_GATE) return INSMOS_EINVAL;
     const int64_t es = size_of(dtype), chunk = 16 / es;
     if (!good_matrix(dy, ld_dy, N, dtype) || (slope_kind == INSMOS_SLOPE_SIGN && !good_matrix(slope, ld_slope, N, dtype)) ||
-        (slope_kind == INSMOS_SLOPE_STORED && (!slope || !good_rows(slope, ld_slope, N, dtype))) || (dx && !good_matrix(dx, ld_dx, K, dtype)) ||
+        (slope_kind >= INSMOS_SLOPE_STORED && (!slope || !good_rows(slope, ld_slope, N, dtype))) || (dx && !good_matrix(dx, ld_dx, K, dtype)) ||
         (dx && !good_matrix(w, ld_w, w_out_in ? K : N, dtype)) || (dw && !good_matrix(x, ld_x, K, dtype)) ||
         (dw && !good_matrix(dw, ld_dw, w_out_in ? K : N, dtype)) || (uintptr_t)db % es || (uintptr_t)ws % 16)
         return INSMOS_EINVAL;
