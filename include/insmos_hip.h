@@ -854,7 +854,7 @@ int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dt
  * pitch >= 0 (0: one row for all), or NULL; y (M, N).  All of one dtype (INSMOS_F32 / BF16 / F16), pitches in elements (at most 2^20, as are
  * K and N); sums in fp32, one rounding per output.  Addresses and pitches need only the elements' alignment; 16-bit operands at odd
  * addresses or pitches are laid out again in ws.  slope: NULL, or receives act'(z) for the backward pass, in fp32 for INSMOS_F32 and otherwise as 16 bits
- * (steps of 2^-15 from -1/2; 0: not a number), 16-byte aligned, ld_slope a multiple of 16 bytes that holds N rounded up to 16 bytes; not
+ * (of the library's own: off by at most 2^-16, and by 2^-10 of itself from 2^-6 down to 2^-28), 16-byte aligned, ld_slope a multiple of 16 bytes that holds N rounded up to 16 bytes; not
  * without an activation.
  * Backward: dz = dy act'(z);  dx = dz W^T;  dw = x^T dz in the weight's layout;  db = column sums of dz (before its rounding to the type).
  * slope_kind: INSMOS_SLOPE_NONE (no activation), INSMOS_SLOPE_SIGN (slope holds y = relu(z), of which the sign counts), INSMOS_SLOPE_STORED

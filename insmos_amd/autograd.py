@@ -515,8 +515,9 @@ def linear(x, weight, bias=None, residual=None, activation=None, residual_first=
     "relu", "gelu" (erf), "gelu_tanh" or "silu".  All tensors of one dtype -- float32, bfloat16 or float16 -- on one GPU; sums in fp32.
     Widths up to 2^20.  Differentiable once in all four tensors, backwards (a forward-mode tangent is refused, and so are torch.func's
     transforms); without gradients nothing is kept for a backward pass.  Tracers, fake tensors and dispatch modes see it as insmos::linear.
-    In 16 bits the backward rounds dz once, for the products.  Forward and backward can be captured into a graph; the backward refuses where
-    a graph that was recorded on the default stream shares its inputs and is still alive."""
+    In 16 bits the backward rounds dz once, for the products (fp16: to its range, so losses are scaled as usual), and takes act' from 16 bits, off
+    by at most 2^-16, and by 2^-10 of itself where it is below 2^-6 (down to 2^-28).  Forward and backward can be captured into a graph; the backward
+    refuses where a graph that was recorded on the default stream shares its inputs and is still alive."""
     try:
         act = _ACTIVATIONS[activation]
     except (KeyError, TypeError):

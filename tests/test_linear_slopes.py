@@ -49,3 +49,61 @@ def test_linear_a_shut_relu_keeps_what_comes_from_behind(dtype, residual):
     db = torch.autograd.grad(y, ins[2], dy)[0]
     want = torch.tensor([40.0, 0.0, 0.0, -float("inf")]).repeat(4).to(t).cuda()
     assert torch.equal(db, want)
+
+
+U32 = 2.0 ** -24
+
+
+def _slope64(z, act):
+    z = z.double().detach().requires_grad_(True)
+    y = torch.nn.functional.silu(z) if act == "silu" else torch.nn.functional.gelu(z, approximate="tanh" if act == "gelu_tanh" else "none")
+    return torch.autograd.grad(y.sum(), z)[0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("act,least", [("silu", -22.0), ("gelu", -6.5), ("gelu_tanh", -5.5)])
+def test_linear_slopes_in_the_tails_keep_their_size(dtype, act, least):
+    """dz against the slope in float64, relative to the slope itself.  Its errors: the 16-bit types' code, 2^-10 of a slope below 2^-6 in size and 2^-16
+    above; the exponential's, whose argument (up to z^2 / 2 or 1.6 |z| + 0.1 |z|^3) is rounded in fp32; where |z| < 3 that of terms of size 1 which
+    nearly cancel; one rounding to the type (fp16: half of its smallest step at least)."""
+    t = DTYPES[dtype]
+    n = 64
+    z = torch.linspace(least, 0.5, 40 * n).view(40, n).to(torch.bfloat16).float()      # exact in every type
+    gen = torch.Generator().manual_seed(3)
+    # gradients of a scaled loss: what fp16 has least of stays small against dz
+    dy = (1024.0 * (1 + torch.rand(40, n, generator=gen))).to(t).cuda()
+    y, ins = _one_each(z, t, act, torch.zeros(40, n), True)
+    dz = torch.autograd.grad(y, ins[3], dy)[0].double()
+    s = _slope64(z.cuda(), act)
+    code = torch.where(s.abs() < 2.0 ** -6, 2.0 ** -10 * s.abs(), torch.full_like(s, 2.0 ** -16)) if dtype != "fp32" else 0
+    arg = 8 * U32 * (1 + z.cuda().double() ** 2 + 0.1 * z.cuda().double().abs() ** 3) * (s.abs() + (z.cuda().abs() < 3))
+    want, e = dy.double() * s, dy.double() * (code + arg) * (1 + 2.0 ** -10)
+    half = torch.finfo(t).eps / 2
+    ok = (dz - want).abs() <= half * want.abs() + (1 + half) * e + (2.0 ** -25 if dtype == "fp16" else 1e-30)
+    assert bool(ok.all()), ((dz - want).abs() / want.abs())[~ok].max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("act,bias", [("silu", -12.0), ("silu", -18.0), ("gelu", -5.0), ("gelu_tanh", -4.5)])
+def test_linear_a_unit_that_is_far_in_the_tail_learns(dtype, act, bias):
+    """A strongly negative bias: the slopes of all rows are small and of one sign.  db (a sum in fp32, rounded once) is off by 2^-10 of the sum, the
+    exponentials' errors and its own rounding; dw and dx take dz rounded to the type once more each."""
+    t = DTYPES[dtype]
+    gen = torch.Generator().manual_seed(5)
+    x, w = (torch.rand(200, 32, generator=gen) * 0.1).to(t).cuda(), (torch.rand(32, 24, generator=gen) * 0.1).to(t).cuda()
+    b = torch.full((24,), bias, dtype=t, device="cuda")
+    dy = (1024.0 * (1 + torch.rand(200, 24, generator=gen))).to(t).cuda()
+    ins = [v.requires_grad_(True) for v in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(linear(*ins, activation=act), ins, dy)
+    X, W, D = x.detach().double(), w.detach().double(), dy.double()
+    z = X @ W + bias
+    dz = D * _slope64(z, act)
+    half = torch.finfo(t).eps / 2
+    # z itself: 34 sums and products of at most 12 + 0.4, and d log(slope) / dz of at most |z| + 1 (gelu_tanh: 1.6 + 0.22 z^2 < 8)
+    rel = 2.0 ** -10 + 8 * U32 * (1 + bias ** 2 + 0.1 * abs(bias) ** 3) + 34 * U32 * (abs(bias) + 1) * 20
+    tiny = 2.0 ** -25 if dtype == "fp16" else 0.0      # (dz in fp16: half of the smallest step)
+    for g, ref, each in ((db, dz.sum(0), 0.0), (dw, X.t() @ dz, X.t() @ (half * dz.abs() + tiny)), (dx, dz @ W.t(), (half * dz.abs() + tiny) @ W.t())):
+        off = (g.double() - ref).abs()
+        assert bool((off <= (half + rel) * (1 + half) * ref.abs() + 200 * U32 * ref.abs() + each * (1 + 2.0 ** -7) + tiny).all()), float((off / ref.abs()).max())
