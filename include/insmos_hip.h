@@ -860,7 +860,8 @@ int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tensors, int dt
  * slope_kind: INSMOS_SLOPE_NONE (no activation), INSMOS_SLOPE_SIGN (slope holds y = relu(z), of which the sign counts), INSMOS_SLOPE_STORED
  * (dy times the stored slope, whatever dy is) or INSMOS_SLOPE_GATE (a relu's stored slopes, 0 or 1: where it is shut dz is 0, whatever dy is).
  * Each of dx, dw, db, dz may be NULL; dz: 16-byte aligned rows like slope's.
- * ws: 16-byte aligned, insmos_linear*_ws_bytes bytes.  M = 0 is no work for insmos_linear and refused by the backward.  Outputs overlap
+ * ws: 16-byte aligned, insmos_linear*_ws_bytes_for bytes for the call's operands (often none: then it may be NULL), or insmos_linear*_ws_bytes for any
+ * operands of these sizes; with less the call is refused before its first launch.  M = 0 is no work for insmos_linear and refused by the backward.  Outputs overlap
  * neither inputs nor each other.
  * ---------------------------------------------------------------------------------------------- */
 #define INSMOS_ACT_NONE 0
@@ -877,6 +878,10 @@ int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int 
                   int64_t ld_res, int residual_first, int act, int64_t M, int K, int N, int dtype, void* y, int64_t ld_y,
                   void* slope, int64_t ld_slope, void* ws, size_t ws_bytes, void* stream);
 size_t insmos_linear_backward_ws_bytes(int64_t M, int K, int N, int dtype);
+/* (the operands' addresses and pitches as in the call; dx, dw, db, dz: whether it has that output) */
+size_t insmos_linear_ws_bytes_for(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, int64_t M, int K, int N, int dtype);
+size_t insmos_linear_backward_ws_bytes_for(const void* dy, int64_t ld_dy, int slope_kind, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                           int w_out_in, int64_t M, int K, int N, int dtype, int dx, int dw, int db, int dz);
 int insmos_linear_backward(const void* dy, int64_t ld_dy, const void* slope, int64_t ld_slope, int slope_kind, const void* x, int64_t ld_x,
                            const void* w, int64_t ld_w, int w_out_in, int64_t M, int K, int N, int dtype, void* dx, int64_t ld_dx, void* dw,
                            int64_t ld_dw, void* db, void* dz, int64_t ld_dz, void* ws, size_t ws_bytes, void* stream);

@@ -182,6 +182,9 @@ SIGNATURES = {
     "insmos_linear_backward_ws_bytes": (c_sz, [c_i64, c_int, c_int, c_int]),
     "insmos_linear_backward": (c_int, [c_vp, c_i64, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_int, c_int, c_int, c_vp,
                                        c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_vp, c_sz, c_vp]),
+    "insmos_linear_ws_bytes_for": (c_sz, [c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_int, c_int, c_int]),
+    "insmos_linear_backward_ws_bytes_for": (c_sz, [c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_i64, c_int, c_i64, c_int, c_int, c_int, c_int,
+                                                   c_int, c_int, c_int]),
     "insmos_grad_sumsq_partials": (c_sz, [c_vp, c_int]),
     "insmos_grad_sumsq": (c_int, [c_vp, c_int, c_int, c_vp, c_i64, c_vp]),
     "insmos_grad_norm": (c_int, [c_vp, c_i64, c_vp, c_vp]),

@@ -500,8 +500,8 @@ def _host():
     if _host_module is None:
         lib = _lib.load()
         from . import _host as m
-        m.bind_linear(*[ctypes.cast(f, ctypes.c_void_p).value for f in (lib.insmos_linear, lib.insmos_linear_ws_bytes,
-                                                                        lib.insmos_linear_backward, lib.insmos_linear_backward_ws_bytes)])
+        m.bind_linear(*[ctypes.cast(f, ctypes.c_void_p).value for f in (lib.insmos_linear, lib.insmos_linear_ws_bytes_for,
+                                                                        lib.insmos_linear_backward, lib.insmos_linear_backward_ws_bytes_for)])
         _host_module = m
     return _host_module
 

@@ -163,11 +163,11 @@ PyObject* opt_table(PyObject*, PyObject* args) {
 
 // ---- linear -----------------------------------------------------------------------------------------------------------------
 decltype(&insmos_linear) g_linear = nullptr;
-decltype(&insmos_linear_ws_bytes) g_linear_ws = nullptr;
+decltype(&insmos_linear_ws_bytes_for) g_linear_ws = nullptr;
 decltype(&insmos_linear_backward) g_backward = nullptr;
-decltype(&insmos_linear_backward_ws_bytes) g_backward_ws = nullptr;
+decltype(&insmos_linear_backward_ws_bytes_for) g_backward_ws = nullptr;
 
-// bind_linear(addresses of insmos_linear, _ws_bytes, _backward, _backward_ws_bytes)
+// bind_linear(addresses of insmos_linear, _ws_bytes_for, _backward, _backward_ws_bytes_for)
 PyObject* bind_linear(PyObject*, PyObject* args) {
     unsigned long long f[4];
     if (!PyArg_ParseTuple(args, "KKKK", &f[0], &f[1], &f[2], &f[3])) return nullptr;
@@ -312,7 +312,7 @@ std::pair<at::Tensor, at::Tensor> forward_of(const Layer& l, bool keep) {
         const Weight wt = weight_of(w);
         Rows rr{};
         if (l.r.defined()) rr = rows_of(l.r, cout, true);
-        const size_t need = g_linear_ws(n, (int)cin, (int)cout, dt);
+        const size_t need = g_linear_ws(xr.t.data_ptr(), xr.ld, wt.t.data_ptr(), wt.ld, wt.out_in, n, (int)cin, (int)cout, dt);
         const at::Tensor ws = need ? at::empty({(int64_t)need}, opt.dtype(at::kByte)) : at::Tensor();
         checked(g_linear(xr.t.data_ptr(), xr.ld, wt.t.data_ptr(), wt.ld, wt.out_in, at_ptr(b), at_ptr(rr.t), rr.ld, l.first, l.act, n, (int)cin, (int)cout, dt,
                          y.data_ptr(), cout, at_ptr(slope), ld, at_ptr(ws), need, stream_of(x)), "insmos_linear");
@@ -337,11 +337,12 @@ Grads backward_of(const at::Tensor& dy, const at::Tensor& slope, const at::Tenso
     if (n && cout) {
         if (need_x || need_w || need_b || need_z) {
             const Rows d = rows_of(dy, cout), xr = rows_of(x, cin);
-            const size_t need = g_backward_ws(n, (int)cin, (int)cout, dt);
-            const at::Tensor ws = at::empty({(int64_t)need}, opt.dtype(at::kByte));
+            const size_t need = g_backward_ws(d.t.data_ptr(), d.ld, kind, xr.t.data_ptr(), xr.ld, wt.t.data_ptr(), wt.ld, wt.out_in, n, (int)cin, (int)cout, dt,
+                                              need_x, need_w, need_b, need_z);
+            const at::Tensor ws = need ? at::empty({(int64_t)need}, opt.dtype(at::kByte)) : at::Tensor();
             checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(slope), kind >= INSMOS_SLOPE_STORED ? ld : cout, kind, xr.t.data_ptr(), xr.ld, wt.t.data_ptr(),
                                wt.ld, wt.out_in, n, (int)cin, (int)cout, dt, at_ptr(g.x), cin, at_ptr(g.w), wt.out_in ? cin : cout, at_ptr(g.b),
-                               at_ptr(g.z), ld, ws.data_ptr(), need, stream_of(x)), "insmos_linear_backward");
+                               at_ptr(g.z), ld, at_ptr(ws), need, stream_of(x)), "insmos_linear_backward");
         }
         if (need_z) g.z = g.z.narrow(1, 0, cout).reshape(dy.sizes());
     } else {

@@ -4,6 +4,7 @@
 //
 // The three products are linear.h's; here is what surrounds them: the choice of tile and of parts of k, the layout of operands that the
 // 16-byte loads cannot take as they are, dz with the column sums (one pass over dy and z), and the argument checks.
+#include <algorithm>
 #include <cmath>
 #include "linear.h"
 
@@ -276,6 +277,29 @@ bool good_matrix(const void* p, int64_t ld, int64_t cols, int dtype) {
 }
 // dz needs a buffer of its own where there is an activation or dy cannot be loaded as it is
 bool needs_dz(const void* dy, int64_t ld_dy, int kind, int dtype) { return kind != INSMOS_SLOPE_NONE || !loadable(dy, ld_dy, dtype); }
+// What a forward call takes of ws: copies of operands that the tiles cannot load (a, b: whether x, W are such), and the parts of k.  plan: the call's.
+size_t forward_need(int64_t M, int K, int N, int dtype, bool a, bool b, int w_out_in, const Plan& plan) {
+    if (plan.tile == FEW) return 0;
+    return (a ? packed_bytes(M, K, dtype) : 0) + (!b ? 0 : w_out_in ? packed_bytes(N, K, dtype) : packed_bytes(K, N, dtype)) + plan_bytes(plan, (int)M, N);
+}
+// What a backward call takes: dz where it has no place of its own, the row blocks' column sums, copies of W and x; and the parts of k, one product's
+// after the other's in the same place.
+struct BackwardNeed { bool dz, sums, w, x; Plan dx, dw; };
+size_t backward_need(int64_t M, int K, int N, int dtype, int w_out_in, const BackwardNeed& n) {
+    const size_t p1 = plan_bytes(n.dx, (int)M, K), p2 = w_out_in ? plan_bytes(n.dw, N, K) : plan_bytes(n.dw, K, N);
+    return (n.dz ? packed_bytes(M, N, dtype) : 0) + (n.sums ? pad256((size_t)slope_plan(M, N, dtype).blocks * N * sizeof(float)) : 0) +
+           (!n.w ? 0 : w_out_in ? packed_bytes(N, K, dtype) : packed_bytes(K, N, dtype)) + (n.x ? packed_bytes(M, K, dtype) : 0) + (p1 > p2 ? p1 : p2);
+}
+Plan dw_plan(int64_t M, int K, int N, int dtype, int w_out_in) { return w_out_in ? plan_for(N, K, (int)M, dtype, false) : plan_for(K, N, (int)M, dtype, false); }
+BackwardNeed backward_needs(const void* dy, int64_t ld_dy, int kind, const void* x, int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, int64_t M, int K, int N,
+                            int dtype, bool dx, bool dw, bool db, bool dz) {
+    const bool own = (dx || dw) && needs_dz(dy, ld_dy, kind, dtype), odd_w = dx && !loadable(w, ld_w, dtype);   // (what the products read of dz is loadable)
+    BackwardNeed n = {own && !dz, db && slope_plan(M, N, dtype).blocks > 1, false, dw && !loadable(x, ld_x, dtype), {FEW, 1}, {FEW, 1}};
+    if (dx) n.dx = plan_for((int)M, K, N, dtype, true, odd_w);
+    n.w = odd_w && n.dx.tile != FEW;
+    if (dw) n.dw = dw_plan(M, K, N, dtype, w_out_in);
+    return n;
+}
 // rows of a buffer in the library's own layout: 16-byte aligned, whole chunks
 bool good_rows(const void* p, int64_t ld, int N, int dtype) {
     const int64_t chunk = 16 / (int64_t)size_of(dtype);
@@ -288,9 +312,17 @@ bool good_rows(const void* p, int64_t ld, int N, int dtype) {
 using namespace insmos;
 using namespace insmos::lin;
 
+// (an operand of 16 bits may be one that is copied; where such a call takes the kernel for few rows, so do all)
 extern "C" size_t insmos_linear_ws_bytes(int64_t M, int K, int N, int dtype) {
     if (!good_shape(M, K, N, dtype) || !M) return 0;
-    return packed_bytes(M, K, dtype) + packed_bytes(K, N, dtype) + packed_bytes(N, K, dtype) + plan_bytes(plan_for((int)M, N, K, dtype, true), (int)M, N);
+    const Plan plan = plan_for((int)M, N, K, dtype, true);
+    const bool odd = dtype != INSMOS_F32;
+    return std::max(forward_need(M, K, N, dtype, odd, odd, 0, plan), forward_need(M, K, N, dtype, odd, odd, 1, plan));
+}
+extern "C" size_t insmos_linear_ws_bytes_for(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, int64_t M, int K, int N, int dtype) {
+    if (!good_shape(M, K, N, dtype) || !M) return 0;
+    const bool a = !loadable(x, ld_x, dtype), b = !loadable(w, ld_w, dtype);
+    return forward_need(M, K, N, dtype, a, b, w_out_in, plan_for((int)M, N, K, dtype, true, a || b));
 }
 extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, const void* bias, const void* residual,
                              int64_t ld_res, int residual_first, int act, int64_t M, int K, int N, int dtype, void* y, int64_t ld_y,
@@ -305,8 +337,9 @@ extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t
     const hipStream_t s = (hipStream_t)stream;
     Bump bump(ws, ws ? ws_bytes : 0);
     Operand a, b;
-    // (with FEW for odd operands less of ws is used than insmos_linear_ws_bytes counted)
-    const Plan plan = plan_for((int)M, N, K, dtype, true, !loadable(x, ld_x, dtype) || !loadable(w, ld_w, dtype));
+    const bool odd_x = !loadable(x, ld_x, dtype), odd_w = !loadable(w, ld_w, dtype);
+    const Plan plan = plan_for((int)M, N, K, dtype, true, odd_x || odd_w);
+    if (bump.cap < forward_need(M, K, N, dtype, odd_x, odd_w, w_out_in, plan)) return INSMOS_EWORKSPACE;   // (before the first launch)
     const bool any = plan.tile == FEW;
     int rc = operand(x, ld_x, M, K, KC, dtype, any, bump, s, &a);
     if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, KC, dtype, any, bump, s, &b) : operand(w, ld_w, K, N, NC, dtype, any, bump, s, &b);
@@ -323,11 +356,17 @@ extern "C" int insmos_linear(const void* x, int64_t ld_x, const void* w, int64_t
 
 extern "C" size_t insmos_linear_backward_ws_bytes(int64_t M, int K, int N, int dtype) {
     if (!good_shape(M, K, N, dtype) || !M) return 0;
-    const SlopePlan r = slope_plan(M, N, dtype);
-    const Plan dx = plan_for((int)M, K, N, dtype, true), dw = plan_for(K, N, (int)M, dtype, false), dwt = plan_for(N, K, (int)M, dtype, false);
-    const size_t w1 = plan_bytes(dw, K, N), w2 = plan_bytes(dwt, N, K);
-    return packed_bytes(M, N, dtype) + pad256((size_t)r.blocks * N * sizeof(float)) + packed_bytes(K, N, dtype) + packed_bytes(N, K, dtype) +
-           packed_bytes(M, K, dtype) + plan_bytes(dx, (int)M, K) + (w1 > w2 ? w1 : w2);
+    const Plan dx = plan_for((int)M, K, N, dtype, true);
+    const bool odd = dtype != INSMOS_F32, sums = slope_plan(M, N, dtype).blocks > 1;
+    size_t need = 0;
+    for (int out_in = 0; out_in < 2; ++out_in)
+        need = std::max(need, backward_need(M, K, N, dtype, out_in, {true, sums, odd && dx.tile != FEW, odd, dx, dw_plan(M, K, N, dtype, out_in)}));
+    return need;
+}
+extern "C" size_t insmos_linear_backward_ws_bytes_for(const void* dy, int64_t ld_dy, int slope_kind, const void* x, int64_t ld_x, const void* w, int64_t ld_w,
+                                                      int w_out_in, int64_t M, int K, int N, int dtype, int dx, int dw, int db, int dz) {
+    if (!good_shape(M, K, N, dtype) || !M) return 0;
+    return backward_need(M, K, N, dtype, w_out_in, backward_needs(dy, ld_dy, slope_kind, x, ld_x, w, ld_w, w_out_in, M, K, N, dtype, dx, dw, db, dz));
 }
 extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void* slope, int64_t ld_slope, int slope_kind, const void* x,
                                       int64_t ld_x, const void* w, int64_t ld_w, int w_out_in, int64_t M, int K, int N, int dtype, void* dx, int64_t ld_dx, void* dw,
@@ -344,6 +383,8 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
     const hipStream_t s = (hipStream_t)stream;
     Bump bump(ws, ws ? ws_bytes : 0);
     int rc = INSMOS_OK;
+    const BackwardNeed needs = backward_needs(dy, ld_dy, slope_kind, x, ld_x, w, ld_w, w_out_in, M, K, N, dtype, dx, dw, db, dz);
+    if (bump.cap < backward_need(M, K, N, dtype, w_out_in, needs)) return INSMOS_EWORKSPACE;   // (before the first launch)
     const void* d = dy;
     int64_t ld_d = ld_dy;
     const bool own = dz || ((dx || dw) && needs_dz(dy, ld_dy, slope_kind, dtype));
@@ -376,16 +417,17 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
     }
     if (dx) {   // (M, K) = dz (M, N) W^T: k of this product is N
         Operand a, b;
-        const Plan plan = plan_for((int)M, K, N, dtype, true, !loadable(d, ld_d, dtype) || !loadable(w, ld_w, dtype));
-        const bool any = plan.tile == FEW;
+        const bool any = needs.dx.tile == FEW;
         rc = operand(d, ld_d, M, N, KC, dtype, any, bump, s, &a);
         if (rc == INSMOS_OK) rc = w_out_in ? operand(w, ld_w, N, K, NC, dtype, any, bump, s, &b) : operand(w, ld_w, K, N, KC, dtype, any, bump, s, &b);
         if (rc != INSMOS_OK) return rc;
         GemmP p = {};
         p.M = (int)M; p.N = K; p.K = N;
         p.y = dx; p.ld_y = ld_dx;
-        rc = run_gemm(p, a, b, dtype, plan, bump, s);
+        const size_t before = bump.off;
+        rc = run_gemm(p, a, b, dtype, needs.dx, bump, s);
         if (rc != INSMOS_OK) return rc;
+        bump.off = before;   // (dw's parts are written behind this product's, on the same stream)
     }
     if (dw) {   // (K, N) = x^T dz, or its transpose for a (N, K) weight: k of this product is M
         Operand a, b;
@@ -395,8 +437,7 @@ extern "C" int insmos_linear_backward(const void* dy, int64_t ld_dy, const void*
         GemmP p = {};
         p.M = w_out_in ? N : K; p.N = w_out_in ? K : N; p.K = (int)M;
         p.y = dw; p.ld_y = ld_dw;
-        const Plan plan = plan_for(p.M, p.N, p.K, dtype, false);
-        rc = w_out_in ? run_gemm(p, b, a, dtype, plan, bump, s) : run_gemm(p, a, b, dtype, plan, bump, s);
+        rc = w_out_in ? run_gemm(p, b, a, dtype, needs.dw, bump, s) : run_gemm(p, a, b, dtype, needs.dw, bump, s);
     }
     return rc;
 }
