@@ -211,10 +211,15 @@ Rows rows_of(const at::Tensor& t, int64_t cols, bool shared = false) {
     return {v, n, n != 1 ? v.stride(0) : cols};
 }
 struct Weight { at::Tensor t; int64_t ld; int out_in; };
+// whether w lies as (cout, cin) rows
+bool out_in_of(const at::Tensor& w) {
+    const auto rows = [&](int d, int64_t cols) { return w.stride(1 - d) == 1 && w.stride(d) >= cols && w.stride(d) <= kMost; };
+    return !rows(0, w.size(1)) && rows(1, w.size(0));
+}
 Weight weight_of(const at::Tensor& w) {
-    const int64_t cin = w.size(0), cout = w.size(1);
+    if (out_in_of(w)) return {w, w.stride(1), 1};
+    const int64_t cout = w.size(1);
     if (w.stride(1) == 1 && w.stride(0) >= cout && w.stride(0) <= kMost) return {w, w.stride(0), 0};
-    if (w.stride(0) == 1 && w.stride(1) >= cin && w.stride(1) <= kMost) return {w, w.stride(1), 1};
     return {w.contiguous(), cout, 0};
 }
 void* at_ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -320,36 +325,43 @@ std::pair<at::Tensor, at::Tensor> forward_of(const Layer& l, bool keep) {
     return {y, slope};
 }
 struct Grads { at::Tensor x, w, b, z; };
-// The gradients that are asked for (z: that of the value before the activation).  kind: INSMOS_SLOPE_*
-Grads backward_of(const at::Tensor& dy, const at::Tensor& slope, const at::Tensor& x, const at::Tensor& w, int kind, bool need_x, bool need_w, bool need_b,
-                  bool need_z) {
-    const int dt = dtype_code(x.scalar_type());
-    const int64_t cin = w.size(0), cout = w.size(1), n = x.numel() / cin, ld = padded(cout, x);
-    if (dy.scalar_type() != x.scalar_type() || dy.device() != x.device()) refuse("the gradient is of another type or device than the output");
-    c10::DeviceGuard guard(x.device());
-    const auto opt = x.options().requires_grad(false);
-    const Weight wt = weight_of(w);
+// The gradients that are asked for (z: that of the value before the activation).  x is read for w's gradient alone and w for x's; out_in: the layout
+// that w's gradient is given in.  kind: INSMOS_SLOPE_*
+Grads backward_of(const at::Tensor& dy, const at::Tensor& slope, const at::Tensor& x, const at::Tensor& w, int64_t cin, bool out_in, int kind, bool need_x, bool need_w,
+                  bool need_b, bool need_z) {
+    const int dt = dtype_code(dy.scalar_type());
+    const int64_t cout = dy.size(-1), n = cout ? dy.numel() / cout : 0, ld = padded(cout, dy);
+    for (const at::Tensor* t : {&x, &w})
+        if (t->defined() && (dy.scalar_type() != t->scalar_type() || dy.device() != t->device())) refuse("the gradient is of another type or device than the output");
+    c10::DeviceGuard guard(dy.device());
+    const auto opt = dy.options().requires_grad(false);
+    std::vector<int64_t> in(dy.sizes().begin(), dy.sizes().end());
+    in.back() = cin;
     Grads g;
-    if (need_x) g.x = at::empty(x.sizes(), opt);
-    if (need_w) g.w = wt.out_in ? at::empty({cout, cin}, opt) : at::empty({cin, cout}, opt);
+    if (need_x) g.x = at::empty(in, opt);
+    if (need_w) g.w = out_in ? at::empty({cout, cin}, opt) : at::empty({cin, cout}, opt);
     if (need_b) g.b = at::empty({cout}, opt);
     if (need_z) g.z = n && cout ? at::empty({n, ld}, opt) : at::empty(dy.sizes(), opt);
     if (n && cout) {
         if (need_x || need_w || need_b || need_z) {
-            const Rows d = rows_of(dy, cout), xr = rows_of(x, cin);
-            const size_t need = g_backward_ws(d.t.data_ptr(), d.ld, kind, xr.t.data_ptr(), xr.ld, wt.t.data_ptr(), wt.ld, wt.out_in, n, (int)cin, (int)cout, dt,
+            const Rows d = rows_of(dy, cout);
+            Rows xr{at::Tensor(), n, cin};
+            if (need_w) xr = rows_of(x, cin);
+            Weight wt{at::Tensor(), out_in ? cin : cout, out_in};
+            if (need_x) wt = weight_of(w);
+            const size_t need = g_backward_ws(d.t.data_ptr(), d.ld, kind, at_ptr(xr.t), xr.ld, at_ptr(wt.t), wt.ld, out_in, n, (int)cin, (int)cout, dt,
                                               need_x, need_w, need_b, need_z);
             const at::Tensor ws = need ? at::empty({(int64_t)need}, opt.dtype(at::kByte)) : at::Tensor();
-            checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(slope), kind >= INSMOS_SLOPE_STORED ? ld : cout, kind, xr.t.data_ptr(), xr.ld, wt.t.data_ptr(),
-                               wt.ld, wt.out_in, n, (int)cin, (int)cout, dt, at_ptr(g.x), cin, at_ptr(g.w), wt.out_in ? cin : cout, at_ptr(g.b),
-                               at_ptr(g.z), ld, at_ptr(ws), need, stream_of(x)), "insmos_linear_backward");
+            checked(g_backward(d.t.data_ptr(), d.ld, at_ptr(slope), kind >= INSMOS_SLOPE_STORED ? ld : cout, kind, at_ptr(xr.t), xr.ld, at_ptr(wt.t), wt.ld, out_in,
+                               n, (int)cin, (int)cout, dt, at_ptr(g.x), cin, at_ptr(g.w), out_in ? cin : cout, at_ptr(g.b), at_ptr(g.z), ld, at_ptr(ws), need,
+                               stream_of(dy)), "insmos_linear_backward");
         }
         if (need_z) g.z = g.z.narrow(1, 0, cout).reshape(dy.sizes());
     } else {
         for (at::Tensor* t : {&g.x, &g.w, &g.b})
             if (t->defined()) t->zero_();
     }
-    if (need_w && wt.out_in) g.w = g.w.t();
+    if (need_w && out_in) g.w = g.w.t();
     return g;
 }
 // A backward pass that is captured into a graph must not reach a node that was recorded on the default stream (a leaf's, kept alive by an eager
@@ -364,16 +376,16 @@ void refuse_default_stream() {
             refuse("a backward pass is being captured, but a graph on the default stream shares its inputs and is alive (drop that graph's outputs before the capture)");
     }
 }
-// The node keeps x, W and the activation's slopes (16 bits each with 16-bit types; y itself for a relu without a residual behind it).
+// The node keeps x where W needs a gradient, W where x does, and the activation's slopes (16 bits each with 16-bit types; y itself for a relu without a residual behind it).
 struct LinearNode : torch::autograd::Function<LinearNode> {
-    enum : int64_t { kFirst = 4, kBias = 8, kResidual = 16 };   // beside the two bits of INSMOS_SLOPE_*
+    enum : int64_t { kFirst = 4, kBias = 8, kResidual = 16, kOutIn = 32, kCin = 8 };   // beside the two bits of INSMOS_SLOPE_*; cin from bit 8 on
     using Maybe = std::optional<at::Tensor>;
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const Maybe& b, const Maybe& r, int64_t act,
                               bool first) {
         const int kind = slope_kind((int)act, r.has_value(), first);
         const auto out = forward_of({x, w, b.value_or(at::Tensor()), r.value_or(at::Tensor()), (int)act, first}, kind >= INSMOS_SLOPE_STORED);
-        ctx->save_for_backward({x, w, kind == INSMOS_SLOPE_SIGN ? out.first : out.second});
-        ctx->saved_data["meta"] = kind + (first ? kFirst : 0) + (b ? kBias : 0) + (r ? kResidual : 0);
+        ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), x.requires_grad() ? w : at::Tensor(), kind == INSMOS_SLOPE_SIGN ? out.first : out.second});
+        ctx->saved_data["meta"] = kind + (first ? kFirst : 0) + (b ? kBias : 0) + (r ? kResidual : 0) + (out_in_of(w) ? kOutIn : 0) + (w.size(0) << kCin);
         return out.first;
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list dys) {
@@ -389,7 +401,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
             const bool need_b = meta & kBias && ctx->needs_input_grad(2), need_r = meta & kResidual && ctx->needs_input_grad(meta & kBias ? 3 : 2);
             const bool z = need_r && meta & kFirst && kind != INSMOS_SLOPE_NONE;
             const at::Tensor dy = dys[0].resolve_neg();
-            const Grads g = backward_of(dy, saved[2], saved[0], saved[1], kind, ctx->needs_input_grad(0), ctx->needs_input_grad(1), need_b, z);
+            const Grads g = backward_of(dy, saved[2], saved[0], saved[1], meta >> kCin, meta & kOutIn, kind, ctx->needs_input_grad(0), ctx->needs_input_grad(1), need_b, z);
             out[0] = g.x;
             out[1] = g.w;
             out[2] = g.b;
@@ -433,8 +445,9 @@ PyObject* linear_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         bool is[5];
         for (int i = 0; i < 5; ++i) is[i] = PyObject_IsTrue(a[5 + i]) == 1;
         const int kind = slope_kind((int)PyLong_AsLong(a[4]), is[0], !is[0]);
-        const Grads g = backward_of(arg(a[0], "the gradient"), a[1] == Py_None ? at::Tensor() : arg(a[1], "slope"), arg(a[2], "x"), arg(a[3], "weight"),
-                                    kind, is[1], is[2], is[3], is[4]);
+        const at::Tensor w = arg(a[3], "weight");
+        const Grads g = backward_of(arg(a[0], "the gradient"), a[1] == Py_None ? at::Tensor() : arg(a[1], "slope"), arg(a[2], "x"), w, w.size(0), out_in_of(w), kind,
+                                    is[1], is[2], is[3], is[4]);
         return Py_BuildValue("NNNN", wrap(g.x), wrap(g.w), wrap(g.b), wrap(g.z));
     });
 }

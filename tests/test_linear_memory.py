@@ -97,3 +97,29 @@ def test_the_reserve_for_any_operands_is_enough(dtype, m, k, n):
                 want = (D @ (W if out_in else W.t()), D.t() @ X if out_in else X.t() @ D, D.sum(0))
                 for g, r in zip((dx, dw, db), want):
                     assert bool((g == 7).all()) if size < exact else torch.equal(g, r.to(t))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", [None, "relu", "gelu"])
+@pytest.mark.parametrize("out_in", [False, True])
+def test_the_tape_keeps_what_the_needed_gradients_read(act, out_in):
+    """x for the weight's gradient, the weight for x's, slopes (relu: y) for any; the gradients are those of the whole set."""
+    gen = torch.Generator().manual_seed(2)
+    x, b, r, dy = (torch.randn(s, generator=gen).cuda() for s in ((40, 24), (16,), (40, 16), (40, 16)))
+    w = torch.randn(16, 24, generator=gen).cuda().t() if out_in else torch.randn(24, 16, generator=gen).cuda()
+
+    def run(needed):
+        kept, ins = [], [t.detach().requires_grad_(i in needed) for i, t in enumerate((x, w, b, r))]
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: (kept.append(t.data_ptr()), t)[1], lambda t: t):
+            y = linear(*ins, activation=act, residual_first=True)
+        grads = torch.autograd.grad(y, [ins[i] for i in needed], dy)
+        return kept, dict(zip(needed, grads)), [t.stride() for t in grads]
+
+    _, want, _ = run((0, 1, 2, 3))
+    for needed in ((0,), (1,), (2,), (3,), (0, 2), (1, 3), (0, 1)):
+        kept, got, strides = run(needed)
+        assert (x.data_ptr() in kept) == (1 in needed) and (w.data_ptr() in kept) == (0 in needed)
+        assert len(kept) == (0 in needed) + (1 in needed) + (act is not None)
+        assert all(torch.equal(got[i], want[i]) for i in needed)
+        if 1 in needed:
+            assert got[1].stride() == w.stride()
