@@ -1,5 +1,7 @@
 """What the backward pass of insmos_amd.autograd.linear makes of the activation's slopes where they are far from 1 and where gradients are not
 finite."""
+import math
+
 import pytest
 import torch
 
@@ -55,9 +57,14 @@ U32 = 2.0 ** -24
 
 
 def _slope64(z, act):
-    z = z.double().detach().requires_grad_(True)
-    y = torch.nn.functional.silu(z) if act == "silu" else torch.nn.functional.gelu(z, approximate="tanh" if act == "gelu_tanh" else "none")
-    return torch.autograd.grad(y.sum(), z)[0]
+    """act'(z) in float64 without the cancellation of 1 + erf and 1 + tanh (which leave 1e-16, 1 % of gelu's slope at -12)."""
+    z = z.double()
+    if act == "gelu":
+        return 0.5 * torch.erfc(-z / math.sqrt(2)) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    c, d = (1.0, 0.0) if act == "silu" else (2 * math.sqrt(2 / math.pi), 0.044715)      # both are z / (1 + exp(-u)), u = c (z + d z^3)
+    u = c * (z + d * z ** 3)
+    s, rest = torch.sigmoid(u), torch.sigmoid(-u)
+    return s + z * s * rest * c * (1 + 3 * d * z * z)
 
 
 @pytest.mark.gpu
@@ -107,3 +114,24 @@ def test_linear_a_unit_that_is_far_in_the_tail_learns(dtype, act, bias):
     for g, ref, each in ((db, dz.sum(0), 0.0), (dw, X.t() @ dz, X.t() @ (half * dz.abs() + tiny)), (dx, dz @ W.t(), (half * dz.abs() + tiny) @ W.t())):
         off = (g.double() - ref).abs()
         assert bool((off <= (half + rel) * (1 + half) * ref.abs() + 200 * U32 * ref.abs() + each * (1 + 2.0 ** -7) + tiny).all()), float((off / ref.abs()).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_linear_slopes_of_far_values(act, dtype):
+    """The gradients of values far out: slope 0 on one side and 1 on the other, finite, where a formula has 0 times infinity.  Nearer ones against
+    float64 (errors as above)."""
+    t = DTYPES[dtype]
+    far = [50.0, -50.0, 1e4, -1e4, 6e4, -6e4] + ([] if dtype == "fp16" else [1e19, -1e19, 2e19, -2e19, 1e30, -1e30, 3e38, -3e38])
+    near = [0.0, -0.0, 12.0, -12.0, 5.0, -5.0, 1.0, -1.0, 0.25, 8.0, -8.0, 20.0, -20.0]
+    z = torch.tensor([far + near + [0.0] * (32 - len(far) - len(near))])
+    y, ins = _one_each(z, t, act, torch.zeros(1, 32), True)
+    dz = torch.autograd.grad(y, ins[3], torch.ones_like(y))[0].double()
+    zs = ins[0].detach().double()
+    s = (zs > 0).double() if act == "relu" else _slope64(zs.clamp(-700, 700), act)    # (from 700 on 0 and 1 to 1e-300)
+    assert bool(dz.isfinite().all())
+    half, arg = torch.finfo(t).eps / 2, 8 * U32 * (1 + zs.clamp(-40, 40) ** 2 + 0.1 * zs.clamp(-40, 40).abs() ** 3) * (s.abs() + (zs.abs() < 3))
+    code = 0 if dtype == "fp32" or act == "relu" else torch.where(s.abs() < 2.0 ** -6, 2.0 ** -10 * s.abs() + 2.0 ** -38, torch.full_like(s, 2.0 ** -16))
+    off = (dz - s).abs()
+    assert bool((off <= half * s.abs() + (1 + half) * (arg + code) + (2.0 ** -25 if dtype == "fp16" else 2.0 ** -126)).all()), off.max()
