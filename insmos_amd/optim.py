@@ -311,31 +311,43 @@ class AdamW(torch.optim.Optimizer):
                 for i, p in enumerate(b.params):
                     self.state[p] = b.entries(i)
 
+    def _check_entries(self, what, got, p):
+        """`got` is a state_dict's state of a parameter like p."""
+        bits = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
+        want = {"step": (torch.int32, (1,)), "exp_avg": (bits, p.shape), "exp_avg_sq": (bits, p.shape)}
+        if self.state_bits == 8:
+            want["scales"] = (torch.float32, (2, -(-p.numel() // STATE_BLOCK)))
+        if self.master_weights and p.dtype != torch.float32:
+            want["master"] = (torch.float32, p.shape)
+        if set(got) != set(want) or any(not torch.is_tensor(got[k]) or got[k].dtype != t or got[k].shape != torch.Size(s) for k, (t, s) in want.items()):
+            raise ValueError(f"AdamW.load_state_dict: the state of parameter {what} is of another kind or shape "
+                             f"(state_bits {self.state_bits}, master_weights {self.master_weights} here)")
+
     def load_state_dict(self, state_dict):
-        """A state_dict() of an AdamW with the same state_bits and master_weights over parameters of the same shapes."""
+        """A state_dict() of an AdamW with the same state_bits and master_weights over parameters of the same shapes.  One that is refused changes nothing."""
         state = state_dict["state"]
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        lists = [[state.get(j) for j in group["params"]] for group in state_dict["param_groups"]]      # (as the groups' parameters)
+        for group, ids, got in zip(self.param_groups, state_dict["param_groups"], lists):
+            for p, j, entries in zip(group["params"], ids["params"], got):
+                if entries is not None:
+                    self._check_entries(j, entries, p)
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})     # (refuses groups of other sizes)
         self._buckets.clear()
         self.state.clear()
-        at = 0
-        for gi, group in enumerate(self.param_groups):
-            index = {id(p): at + i for i, p in enumerate(group["params"])}
-            at += len(index)
-            if not any(j in state for j in index.values()):
+        for gi, (group, got) in enumerate(zip(self.param_groups, lists)):
+            if all(entries is None for entries in got):
                 continue
+            entries_of = {id(p): entries for p, entries in zip(group["params"], got)}
             for b in self._group_buckets(gi):
                 steps = [0] * len(b.params)
                 for i, p in enumerate(b.params):
-                    got, have = state.get(index[id(p)]), b.entries(i)
-                    if got is None:
+                    entries = entries_of[id(p)]
+                    if entries is None:
                         continue
-                    if set(got) != set(have) or any(got[k].shape != have[k].shape or got[k].dtype != have[k].dtype for k in have):
-                        raise ValueError(f"AdamW.load_state_dict: the state of parameter {index[id(p)]} is of another kind or shape "
-                                         f"(state_bits {self.state_bits}, master_weights {self.master_weights} here)")
-                    steps[i] = int(got["step"])
-                    for k in have:
+                    steps[i] = int(entries["step"])
+                    for k, t in b.entries(i).items():
                         if k != "step":
-                            have[k].copy_(got[k])
+                            t.copy_(entries[k])
                 b.set_steps(steps)
                 for i, p in enumerate(b.params):
                     self.state[p]["step"] = b.steps[b.counter[i]]

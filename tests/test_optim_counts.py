@@ -108,3 +108,55 @@ def test_a_captured_step_counts_for_its_parameters():
         assert [int(o.state[p]["step"]) for p in ps] == [5, 1, 5]
         runs.append([p.detach().clone() for p in ps])
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def _state(params, bits, steps):
+    """A state_dict's state of these parameters with recognisable values."""
+    out, at = {}, 0
+    for i, p in enumerate(params):
+        m = torch.full(p.shape, float(i + 1))
+        out[i] = {"step": torch.tensor([steps[i]], dtype=torch.int32), "exp_avg": m, "exp_avg_sq": m * 2}
+        if bits == 8:
+            out[i] = {**{k: v.to(torch.float8_e4m3fn) if k != "step" else v for k, v in out[i].items()},
+                      "scales": torch.full((2, -(-p.numel() // 256)), 0.5)}
+    return out
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_state_dict_changes_nothing(bits):
+    """Whatever is wrong with a state_dict is found before the state that is there is touched: the last parameter's shape, its kind of state, a missing
+    entry, another optimiser's state, groups of other sizes."""
+    ps = [torch.zeros(s, requires_grad=True) for s in SHAPES]
+    o = AdamW([{"params": ps[:4]}, {"params": ps[4:]}], lr=1e-3, state_bits=bits)
+    groups = o.state_dict()["param_groups"]
+    good = _state(ps, bits, [3, 1, 3, 0, 7, 7, 2])
+    o.load_state_dict({"state": good, "param_groups": groups})
+
+    def same():
+        have = o.state_dict()
+        return have["param_groups"] == groups and all(torch.equal(have["state"][i][k].view(torch.uint8), t.view(torch.uint8)) for i in good for k, t in good[i].items())
+
+    assert same() and [int(o.state[p]["step"]) for p in ps] == [3, 1, 3, 0, 7, 7, 2]
+    last, other = len(ps) - 1, _state(ps, 40 - bits, [5] * 7)
+    shape = _state([*ps[:-1], torch.zeros(10)], bits, [5] * 7)
+    missing = {**_state(ps, bits, [5] * 7), last: {k: t for k, t in good[last].items() if k != "exp_avg_sq"}}
+    foreign = {**_state(ps, bits, [5] * 7), last: {**good[last], "step": torch.tensor(3.0)}}
+    warmer = [{**g, "lr": 9.0} for g in groups]
+    for state in (other, shape, missing, foreign):
+        with pytest.raises(ValueError):
+            o.load_state_dict({"state": state, "param_groups": warmer})
+        assert same()
+    for bad in (warmer[:1], [warmer[0], {**warmer[1], "params": [4, 5]}]):
+        with pytest.raises(ValueError):
+            o.load_state_dict({"state": _state(ps, bits, [5] * 7), "param_groups": bad})
+        assert same()
+
+
+def test_a_state_dict_goes_by_the_numbers_of_its_groups():
+    """Parameters are matched through the groups' lists, as torch.optim does, and ones without state start anew."""
+    ps = [torch.zeros(4, requires_grad=True) for _ in range(3)]
+    o = AdamW(ps, lr=1e-3)
+    state = _state(ps, 32, [1, 2, 3])
+    del state[1]
+    o.load_state_dict({"state": state, "param_groups": [{**o.state_dict()["param_groups"][0], "params": [2, 1, 0]}]})
+    assert [int(o.state[p]["step"]) for p in ps] == [3, 0, 1] and [float(o.state[p]["exp_avg"][0]) for p in ps] == [3.0, 0.0, 1.0]
