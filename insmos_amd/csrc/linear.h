@@ -733,6 +733,8 @@ template <class T, int LA, int LB, int BM, int BN, int WM, int WN>
 int launch_tile(const GemmP& p, int most, hipStream_t s) {
     const int64_t items = (int64_t)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN) * p.splits;
     if (items > 0x7FFFFFFF) return INSMOS_EINVAL;
+    ProfScope ps(KK_LINEAR, s);
+    ps.meta[0] = p.M; ps.meta[1] = p.N; ps.meta[2] = p.K; ps.meta[3] = p.splits;
     const auto kernel = k_linear_gemm<T, LA, LB, BM, BN, WM, WN>;
     INSMOS_LAUNCH(kernel, dim3((unsigned)(items < most ? items : most)), dim3(64 * WM * WN), 0, s, p);
     HIP_TRY(hipGetLastError());
@@ -748,6 +750,8 @@ int launch_gemm_l(const GemmP& p, int tile, hipStream_t s) {
     int rc = INSMOS_EINVAL;
     if constexpr (LA == KC) {
         if (tile == FEW) {
+            ProfScope ps(KK_LINEAR, s);
+            ps.meta[0] = p.M; ps.meta[1] = p.N; ps.meta[2] = p.K; ps.meta[3] = 1;
             const auto kernel = k_linear_few<T, LB>;
             INSMOS_LAUNCH(kernel, dim3((unsigned)((p.N + 31) / 32)), dim3(512), 0, s, p);
             HIP_TRY(hipGetLastError());
@@ -765,6 +769,7 @@ int launch_gemm_l(const GemmP& p, int tile, hipStream_t s) {
     if (tile == T32X128) rc = launch_tile<T, LA, LB, 32, 128, 1, 4>(p, 1024, s);
     if (rc != INSMOS_OK || p.splits == 1) return rc;
     const int64_t rows8 = (int64_t)p.M * (p.ld_part / 8);
+    ProfScope ps(KK_LINEAR, s);
     // many parts are few results: 16 lanes each (469 parts of 64 x 128 fp32: 129 -> 9 us)
     if (p.splits >= 16) {
         const auto kernel = k_linear_join<T, 16>;

@@ -53,6 +53,7 @@ int operand(const void* p, int64_t ld, int64_t rows, int cols, int lay, int dtyp
     if (!d) return INSMOS_EWORKSPACE;
     const int64_t groups = (rows * (to / (16 / es)) + 255) / 256;
     const dim3 grid((unsigned)(groups < 1 << 22 ? groups : 1 << 22)), block(256);
+    ProfScope ps(KK_LINEAR, s);
     INSMOS_LAUNCH(k_linear_pack, grid, block, 0, s, (const uint16_t*)p, ld, rows, cols, (uint16_t*)d, to);
     HIP_TRY(hipGetLastError());
     *out = {d, to, lay};
@@ -258,9 +259,13 @@ int run_slope_t(const SlopeP& p, const SlopePlan& r, void* db, hipStream_t s) {
     const auto kernel = p.kind == INSMOS_SLOPE_STORED ? k_linear_slope<T, INSMOS_SLOPE_STORED>
                         : p.kind == INSMOS_SLOPE_GATE ? k_linear_slope<T, INSMOS_SLOPE_GATE>
                         : p.kind == INSMOS_SLOPE_SIGN ? k_linear_slope<T, INSMOS_SLOPE_SIGN> : k_linear_slope<T, INSMOS_SLOPE_NONE>;
-    INSMOS_LAUNCH(kernel, dim3(r.strips, r.blocks), dim3(256), 0, s, p);
-    HIP_TRY(hipGetLastError());
+    {
+        ProfScope ps(KK_LINEAR_SLOPE, s);
+        INSMOS_LAUNCH(kernel, dim3(r.strips, r.blocks), dim3(256), 0, s, p);
+        HIP_TRY(hipGetLastError());
+    }
     if (p.part) {
+        ProfScope ps(KK_LINEAR_SLOPE, s);
         const auto sum = k_linear_colsum<T>;
         INSMOS_LAUNCH(sum, dim3((p.N + 15) / 16), dim3(1024), 0, s, (const float*)p.part, r.blocks, p.N, p.ld_part, (T*)db);
         HIP_TRY(hipGetLastError());

@@ -424,6 +424,7 @@ int each_launch(const InsmosOptTensor* tensors, int n_tensors, int64_t chunk, bo
 
 template <class T>
 int launch_sumsq(const NormList& L, uint32_t blocks, double* partial, hipStream_t s) {
+    ProfScope ps(KK_ADAMW, s);
     const auto kernel = k_grad_sumsq<T>;
     INSMOS_LAUNCH(kernel, dim3(blocks), dim3(256), 0, s, L, partial);
     HIP_TRY(hipGetLastError());
@@ -442,6 +443,7 @@ int sumsq(const InsmosOptTensor* tensors, int n, int dtype, double* partial, hip
 }
 template <class T, bool MASTER>
 int launch_step(const StepList& L, uint32_t blocks, const StepP& P, int bits, hipStream_t s) {
+    ProfScope ps(KK_ADAMW, s);
     const auto kernel = bits == 32 ? k_adamw<T, MASTER> : k_adamw8<T, MASTER>;
     INSMOS_LAUNCH(kernel, dim3(blocks), dim3(256), 0, s, L, P);
     HIP_TRY(hipGetLastError());
@@ -479,6 +481,7 @@ extern "C" int insmos_grad_sumsq(const InsmosOptTensor* tensors_host, int n_tens
 }
 extern "C" int insmos_grad_norm(const double* partials, int64_t n_partials, float* norm, void* stream) {
     if (n_partials < 0 || (n_partials && !partials) || !norm) return INSMOS_EINVAL;
+    ProfScope ps(KK_ADAMW, (hipStream_t)stream);
     INSMOS_LAUNCH(k_grad_norm, dim3(1), dim3(1024), 0, (hipStream_t)stream, partials, n_partials, norm);
     HIP_TRY(hipGetLastError());
     return INSMOS_OK;
@@ -520,8 +523,11 @@ extern "C" int insmos_adamw_step(const InsmosOptTensor* tensors_host, int n_tens
     Q.seed = seed;
     Q.step = step;
     Q.vals = vals;
-    INSMOS_LAUNCH(k_adamw_prepare, dim3(1), dim3(1024), 0, s, Q);
-    HIP_TRY(hipGetLastError());
+    {
+        ProfScope ps(KK_ADAMW, s);
+        INSMOS_LAUNCH(k_adamw_prepare, dim3(1), dim3(1024), 0, s, Q);
+        HIP_TRY(hipGetLastError());
+    }
     StepP P = {};
     P.vals = vals;
     P.m = exp_avg; P.v = exp_avg_sq; P.scales = scales; P.n_blocks = n_state / OPT_BLOCK;

@@ -123,3 +123,27 @@ def test_the_tape_keeps_what_the_needed_gradients_read(act, out_in):
         assert all(torch.equal(got[i], want[i]) for i in needed)
         if 1 in needed:
             assert got[1].stride() == w.stride()
+
+
+@pytest.mark.gpu
+def test_the_profiler_sees_the_layer_and_the_optimiser():
+    import ctypes
+
+    from insmos_amd.optim import AdamW
+    lib = _lib.load()
+    x, w = torch.randn(300, 40, device="cuda"), torch.randn(40, 24, device="cuda", requires_grad=True)
+    opt = AdamW([w], lr=1e-3, max_grad_norm=1.0)
+    torch.cuda.synchronize()
+    lib.insmos_prof_reset()
+    lib.insmos_prof_enable(1)
+    try:
+        linear(x, w, activation="gelu").sum().backward()
+        opt.step()
+        ids, ms, counts = (ctypes.c_int * 64)(), (ctypes.c_double * 64)(), (ctypes.c_int64 * 64)()
+        n = lib.insmos_prof_read(64, ids, ms, counts)
+    finally:
+        lib.insmos_prof_enable(0)
+    seen = {lib.insmos_prof_name(ids[i]).decode(): counts[i] for i in range(n) if counts[i]}
+    lib.insmos_prof_reset()
+    assert set(seen) == {"linear", "linear_slope", "adamw"}
+    assert seen["linear"] in (2, 3, 4) and seen["linear_slope"] == 1 and seen["adamw"] == 3     # products and joins; dz; norm, values, update
