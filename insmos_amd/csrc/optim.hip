@@ -62,6 +62,7 @@ typedef float of32x4 __attribute__((ext_vector_type(4)));
 typedef float of32x8 __attribute__((ext_vector_type(8)));
 template <class T, int V> struct VecOf { typedef T t __attribute__((ext_vector_type(V))); };
 
+// A published mixer of 32 bits (C. Wellons, 2018: shifts and factors found by a search for the least bias), over position, step and seed.
 __device__ __forceinline__ uint32_t mix32(uint32_t x) {
     x ^= x >> 16; x *= 0x7FEB352Du;
     x ^= x >> 15; x *= 0x846CA68Bu;
