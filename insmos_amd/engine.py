@@ -13,6 +13,7 @@ UR blocks and the instance one-hots) are free: producers write into column slice
 """
 import ctypes
 import os
+import threading
 
 import numpy as np
 import torch
@@ -74,6 +75,9 @@ def _pad4(c):
 def _padc(c):
     """Channel widths insmos_sparse_conv accepts: 4, 8, or a multiple of 16 (zero-padded columns)."""
     return 4 if c <= 4 else 8 if c <= 8 else (c + 15) // 16 * 16
+
+
+_CTX_LOCK = threading.Lock()
 
 
 class _NativeCtx:
@@ -947,35 +951,40 @@ class Engine:
 
     # ------------------------------------------------------------------------------------------------
     def _native_ctx(self):
-        """The immutable C++ context (layer table + config) -- built once, shared by clones."""
-        if self._ctx_box[0] is None:
-            cfgs = _lib.NetCfg()
-            cfgs.w0_const, cfgs.b0_const = self.w0_const.data_ptr(), self.b0_const.data_ptr()
-            cfgs.nbr_bev = self.nbr_bev.data_ptr()
-            cfgs.vs[:] = self.vs
-            cfgs.dt = self.dt
-            cfgs.range[:] = self.range
-            cfgs.score_thresh, cfgs.nms_thresh, cfgs.out_factor = self.score_thresh, self.nms_thresh, self.out_factor
-            cfgs.tvs[:] = self.tvs[:2]
-            cfgs.in_ch, cfgs.ncls, cfgs.max_voxels, cfgs.max_points = self.in_ch, self.ncls, self.max_voxels, self.max_points
-            for l in (1, 2, 3, 4, 5):
-                cfgs.shape[l][:] = self.shape[l]
-            cfgs.bevD, cfgs.bevH, cfgs.bevW, cfgs.nbev = self.bevD, self.bevH, self.bevW, self.nbev
-            cfgs.n_bev_layers, cfgs.up_ch, cfgs.head_ld = self.n_bev_layers, self.up_ch, self.head_ld
-            cfgs.pre_max, cfgs.post_max, cfgs.quirk_exact = self.pre_max, self.post_max, 1 if self.quirk_exact else 0
-            names = sorted(self.L)
-            arr_n = (ctypes.c_char_p * len(names))(*[n.encode() for n in names])
-            arr_l = (_lib.ConvW * len(names))()
-            for i, n in enumerate(names):
-                l = self.L[n]
-                arr_l[i].w, arr_l[i].b, arr_l[i].K, arr_l[i].cin, arr_l[i].cout = l.w.data_ptr(), l.b.data_ptr(), l.K, l.cin, l.cout
-            ctx = ctypes.c_void_p()
-            _lib.check(self.lib.insmos_ctx_create(ctypes.byref(cfgs), arr_n, arr_l, len(names), ctypes.byref(ctx)),
-                       "insmos_ctx_create")
-            # the holder frees the C++ object when the last engine (or clone) that can still run on it lets go of the box;
-            # it also keeps the device tensors the context points at alive for as long as the context exists
-            self._ctx_box[0] = _NativeCtx(self.lib, ctx, (self.L, self.w0_const, self.b0_const, self.nbr_bev))
-        return self._ctx_box[0].handle
+        """The holder of the immutable C++ context (layer table + config) -- built once, shared by clones.  A caller keeps the holder for as
+        long as it runs on the handle: the last reference destroys the context."""
+        with _CTX_LOCK:   # (the first forward of several clones, each on a thread of its own: one builds it, the others wait)
+            if self._ctx_box[0] is None:
+                self._ctx_box[0] = self._make_native_ctx()
+            return self._ctx_box[0]
+
+    def _make_native_ctx(self):
+        cfgs = _lib.NetCfg()
+        cfgs.w0_const, cfgs.b0_const = self.w0_const.data_ptr(), self.b0_const.data_ptr()
+        cfgs.nbr_bev = self.nbr_bev.data_ptr()
+        cfgs.vs[:] = self.vs
+        cfgs.dt = self.dt
+        cfgs.range[:] = self.range
+        cfgs.score_thresh, cfgs.nms_thresh, cfgs.out_factor = self.score_thresh, self.nms_thresh, self.out_factor
+        cfgs.tvs[:] = self.tvs[:2]
+        cfgs.in_ch, cfgs.ncls, cfgs.max_voxels, cfgs.max_points = self.in_ch, self.ncls, self.max_voxels, self.max_points
+        for l in (1, 2, 3, 4, 5):
+            cfgs.shape[l][:] = self.shape[l]
+        cfgs.bevD, cfgs.bevH, cfgs.bevW, cfgs.nbev = self.bevD, self.bevH, self.bevW, self.nbev
+        cfgs.n_bev_layers, cfgs.up_ch, cfgs.head_ld = self.n_bev_layers, self.up_ch, self.head_ld
+        cfgs.pre_max, cfgs.post_max, cfgs.quirk_exact = self.pre_max, self.post_max, 1 if self.quirk_exact else 0
+        names = sorted(self.L)
+        arr_n = (ctypes.c_char_p * len(names))(*[n.encode() for n in names])
+        arr_l = (_lib.ConvW * len(names))()
+        for i, n in enumerate(names):
+            l = self.L[n]
+            arr_l[i].w, arr_l[i].b, arr_l[i].K, arr_l[i].cin, arr_l[i].cout = l.w.data_ptr(), l.b.data_ptr(), l.K, l.cin, l.cout
+        ctx = ctypes.c_void_p()
+        _lib.check(self.lib.insmos_ctx_create(ctypes.byref(cfgs), arr_n, arr_l, len(names), ctypes.byref(ctx)),
+                   "insmos_ctx_create")
+        # the holder frees the C++ object when the last engine (or clone) that can still run on it lets go of the box;
+        # it also keeps the device tensors the context points at alive for as long as the context exists
+        return _NativeCtx(self.lib, ctx, (self.L, self.w0_const, self.b0_const, self.nbr_bev))
 
     def _forward_native(self, pts):
         return self.forward_windows([pts])[0][:2]
@@ -995,7 +1004,7 @@ class Engine:
         if any(p.stride(0) != ld for p in pts_list):
             pts_list = [p[:, :5].contiguous() for p in pts_list]
             ld = 5
-        ctx = self._native_ctx()
+        ctx = self._native_ctx()   # (held until the call below is done with it)
         N = sum(int(p.shape[0]) for p in pts_list)
         if self._arena is None:
             self._arena = torch.empty(900 * N + (256 << 20), dtype=torch.uint8, device=self.device)   # (generous: a retry repeats launches)
@@ -1003,7 +1012,7 @@ class Engine:
         win_n = (ctypes.c_int64 * B)(*[int(p.shape[0]) for p in pts_list])
         outs = (_lib.ForwardOut * B)()
         for _ in range(12):
-            rc = self.lib.insmos_forward_windows(ctx, win_ptr, win_n, B, ld, self._arena.data_ptr(), self._arena.numel(),
+            rc = self.lib.insmos_forward_windows(ctx.handle, win_ptr, win_n, B, ld, self._arena.data_ptr(), self._arena.numel(),
                                                  self._stream(), outs)
             if rc != -3:  # INSMOS_EWORKSPACE: grow the arena and retry
                 break

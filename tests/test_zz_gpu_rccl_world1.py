@@ -129,13 +129,6 @@ def _bench_line(extra):
     return lines[0], out
 
 
-# One run of the whole suite ended in a GPU memory fault while the first of these two was running (a process of its own: bench.py over small windows,
-# all of its memory allocated after the RCCL communicator).  Reading the kernels of that path has not shown the cause, so the workload that both
-# share stays off.
-_FAULTED = pytest.mark.skip(reason="bench.py over these small windows faulted the GPU once; the cause is not shown yet")
-
-
-@_FAULTED
 def test_bench_rccl_selfcheck_runs_the_headline_inside_a_one_rank_nccl_group():
     j, out = _bench_line(["--rccl-selfcheck"])
     assert "backend nccl" in out                       # the backend the process group reported, printed at start-up
@@ -144,7 +137,6 @@ def test_bench_rccl_selfcheck_runs_the_headline_inside_a_one_rank_nccl_group():
     assert j["confusion_points"] == 2 * 4 * j["config"]["current_points"]
 
 
-@_FAULTED
 def test_bench_default_line_carries_the_rccl_world1_leg():
     j, _ = _bench_line([])
     leg = j["rccl_world1"]
