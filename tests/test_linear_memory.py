@@ -147,3 +147,28 @@ def test_the_profiler_sees_the_layer_and_the_optimiser():
     lib.insmos_prof_reset()
     assert set(seen) == {"linear", "linear_slope", "adamw"}
     assert seen["linear"] in (2, 3, 4) and seen["linear_slope"] == 1 and seen["adamw"] == 3     # products and joins; dz; norm, values, update
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("m,k,n", [(1, 40, 24), (5, 130, 33), (33, 64, 40), (300, 72, 65), (300, 520, 514), (1000, 40, 8), (61, 700, 2050), (2100, 264, 72), (4100, 2050, 30)])
+def test_what_lies_around_the_operands_is_not_used(dtype, m, k, n):
+    """Every operand as a block of a larger matrix of NaN: rows before and behind it, columns on both sides.  Whole numbers, so results are exact."""
+    t, gen = getattr(torch, dtype), torch.Generator().manual_seed(m)
+
+    def block(rows, cols, left, right):
+        hold = torch.full((rows + 200, cols + left + right), float("nan"), dtype=t, device="cuda")
+        v = hold[100:100 + rows, left:left + cols]
+        v.copy_(torch.randint(-2, 3, (rows, cols), generator=gen))
+        return v
+
+    for left, right in ((8, 8), (2, 6), (1, 2)):
+        for out_in in (False, True):
+            x, r, dy = block(m, k, left, right), block(m, n, left, right), block(m, n, left, right)
+            w = block(n, k, left, right).t() if out_in else block(k, n, left, right)
+            ins = [v.detach().requires_grad_(True) for v in (x, w, r)]
+            y = linear(ins[0], ins[1], None, ins[2])
+            dx, dw, dr = torch.autograd.grad(y, ins, dy)
+            X, W, R, D = (v.double() for v in (x, w, r, dy))
+            for got, want in ((y, X @ W + R), (dx, D @ W.t()), (dw, X.t() @ D), (dr, D)):
+                assert torch.equal(got.detach(), want.to(t)), (left, right, out_in)
