@@ -114,10 +114,11 @@ def pmc_traffic(args, wpl, cfg="cfg2", profiles_dir=None, lib_hash=None):
     launch-set size; stale = True when the latest pass was taken from ANOTHER binary than the one loaded now (its `lib_source_hash`
     differs from insmos_amd/libinsmos_hip.so.srchash, or it carries none) -- the line then prints traffic: null, traffic_stale: true."""
     suffix = "" if cfg == "cfg2" else "_" + cfg
-    cands = sorted(glob.glob(os.path.join(profiles_dir or os.path.join(ROOT, "profiles"), "r0*_pmc_traffic%s.json" % suffix)))
+    where = profiles_dir or os.path.join(ROOT, "profiles")
+    cands = sorted(glob.glob(os.path.join(where, "r0*_pmc_traffic%s.json" % suffix))) + glob.glob(os.path.join(where, "pmc_traffic%s.json" % suffix))
     if not cands or (cfg == "cfg2" and args.n_az != 1886):
         return None, False
-    path = cands[-1]   # the latest round's passes
+    path = cands[-1]   # the latest passes
     with open(path) as f:
         j = json.load(f)
     if int(j.get("windows_per_launch", -1)) != int(wpl):

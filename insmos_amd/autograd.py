@@ -551,6 +551,8 @@ def _slopes_of(activation, residual_behind):
 
 @_linear_op.register_fake
 def _(x, weight, bias, residual, activation, residual_first):
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"linear: x (..., cin) and weight (cin, cout), not {tuple(x.shape)} and {tuple(weight.shape)}")
     y = x.new_empty((*x.shape[:-1], weight.shape[1]))
     if not _slopes_of(activation, residual is not None and not residual_first):
         return y, x.new_empty(0)

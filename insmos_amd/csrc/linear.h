@@ -295,9 +295,9 @@ struct Frag {
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 };
-// fp32: four steps of 32x32x2 take the k of 8 in the order 0 2 | 4 6 | 1 3 | 5 7 (the lower half of the lanes has the first of each pair).  That
-// is the order in which 16x16x4 instructions over 8-byte pieces add, which is how the platform's fp32 product usually sums: the two then agree
-// to the last bit, and so do a relu's decisions at its border.
+// fp32: four steps of 32x32x2 take the k of 8 in the order 0 2 | 4 6 | 1 3 | 5 7 (the lower half of the lanes has the first of each pair), so that a
+// KC fragment is two 8-byte reads.  (The kernel for few rows and products in parts add in other orders; a z within their rounding of a relu's
+// border may be decided either way.)
 template <int LAY, int R, int NT>
 struct Frag<float, LAY, R, NT> {
     typedef f32x4 type;
@@ -473,7 +473,7 @@ struct Gemm {
 
 // Workgroup w runs on XCD w % 8 (each has an L2 of its own), so every XCD gets a contiguous run of items, walked in groups of 8 tile rows: the
 // operands of the tiles in flight on one XCD stay in its L2 (groups of 4, 8 or 16: within 3 %).  Bound by the matrix units from a K of some hundreds
-// on: 8192 x 4096 x 8192 bf16 with gelu_tanh and a residual 486 .. 496 us = 1110 .. 1131 TFLOP/s (the platform's plain product: 1186), 4096^3 fp32 982 us = 140 of
+// on: 8192 x 4096 x 8192 bf16 with gelu_tanh and a residual 478 .. 494 us = 1113 .. 1150 TFLOP/s (the platform's plain product: 1186), 4096^3 fp32 982 us = 140 of
 // 157; below that by the epilogue's lines and vector work (some 12 us per 256 x 256 tile, 8 for two of 128 x 128 side by side).
 template <class T, int LA, int LB, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, 2) k_linear_gemm(const GemmP p) {

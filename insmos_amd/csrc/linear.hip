@@ -3,7 +3,7 @@
 //   dz = dy act'(z);   dx = dz W^T;   dW = x^T dz;   db = sum over rows of dz;   dr = dz (residual first) or dy
 //
 // The three products are linear.h's; here is what surrounds them: the choice of tile and of parts of k, the layout of operands that the
-// 16-byte loads cannot take as they are, dz with the column sums (one pass over dy and z), and the argument checks.
+// 16-byte loads cannot take as they are, dz with the column sums (one pass over dy and the slopes), and the argument checks.
 #include <algorithm>
 #include <cmath>
 #include "linear.h"
@@ -139,7 +139,7 @@ struct SlopeP {
     int lanes;           // column lanes (a power of two <= 32)
 };
 // 256 lanes = `lanes` over the columns (16 bytes each) x the rest over rows; dz rounds dy act'(z) once to the type (the products read it in that
-// type); the column sums are taken before the rounding, in fp32, rows in a fixed order.  Bound by HBM: 8192 x 8192 bf16 87 us (4.6 TB/s for dy, slopes
+// type); the column sums are taken before the rounding, in fp32, rows in a fixed order.  Bound by HBM: 8192 x 8192 bf16 89 us (4.5 TB/s for dy, slopes
 // and dz), 119817 x 128 fp32 30 us (6.1); four rows per lane are in flight.
 template <class T, int KIND>
 __global__ void __launch_bounds__(256) k_linear_slope(const SlopeP p) {

@@ -38,6 +38,8 @@ def test_linear_on_fake_tensors(act, first, out_in):
         x, w, b, r = (torch.empty(s, dtype=torch.bfloat16).requires_grad_() for s in ((5, 4, 24), (16, 24) if out_in else (24, 16), (16,), (5, 4, 16)))
         y = linear(x, w.t() if out_in else w, b, r, activation=act, residual_first=first)
         grads = torch.autograd.grad(y, (x, w, b, r), torch.empty_like(y))
+        with pytest.raises(ValueError, match="weight"):
+            linear(x, torch.empty((23, 16), dtype=torch.bfloat16))
     assert isinstance(y, FakeTensor) and y.shape == (5, 4, 16) and y.dtype == torch.bfloat16
     for g, t in zip(grads, (x, w, b, r)):
         assert isinstance(g, FakeTensor) and g.shape == t.shape and g.dtype == t.dtype
