@@ -67,25 +67,50 @@ int dtype_code(c10::ScalarType t) {
     return t == c10::ScalarType::Float ? INSMOS_F32 : t == c10::ScalarType::BFloat16 ? INSMOS_BF16 : t == c10::ScalarType::Half ? INSMOS_F16 : -1;
 }
 
+void add_order(uint64_t& h, const at::Tensor& t) {
+    auto add = [&](int64_t v) { h = (h ^ (uint64_t)v) * 0x100000001B3u; };
+    add(t.dim());
+    for (int64_t d = 0; d < t.dim(); ++d) {
+        add(t.size(d));
+        add(t.stride(d));
+    }
+}
+constexpr uint64_t kOrder = 0xCBF29CE484222325u;
 // opt_order(params) -> a hash of the tensors' sizes and strides
 PyObject* opt_order(PyObject*, PyObject* list) {
     if (!PyList_Check(list)) { PyErr_SetString(PyExc_ValueError, "opt_order: params is a list"); return nullptr; }
-    uint64_t h = 0xCBF29CE484222325u;
-    auto add = [&](int64_t v) { h = (h ^ (uint64_t)v) * 0x100000001B3u; };
+    uint64_t h = kOrder;
     try {
-        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
-            const at::Tensor& t = tensor_at(list, i, "opt_order", "parameter");
-            add(t.dim());
-            for (int64_t d = 0; d < t.dim(); ++d) {
-                add(t.size(d));
-                add(t.stride(d));
-            }
-        }
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) add_order(h, tensor_at(list, i, "opt_order", "parameter"));
     } catch (const std::exception& e) {
         PyErr_SetString(PyExc_ValueError, e.what());
         return nullptr;
     }
     return PyLong_FromUnsignedLongLong(h);
+}
+// opt_grads(params) -> (that hash, the parameters' gradients, how many have none)
+PyObject* opt_grads(PyObject*, PyObject* list) {
+    if (!PyList_Check(list)) { PyErr_SetString(PyExc_ValueError, "opt_grads: params is a list"); return nullptr; }
+    uint64_t h = kOrder;
+    Py_ssize_t missing = 0;
+    PyObject* grads = PyList_New(PyList_GET_SIZE(list));
+    if (!grads) return nullptr;
+    try {
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+            const at::Tensor& t = tensor_at(list, i, "opt_grads", "parameter");
+            add_order(h, t);
+            PyObject* o = PyList_GET_ITEM(list, i);
+            PyObject* g = THPVariable_CheckExact(o) ? THPVariable_Wrap(t.grad()) : PyObject_GetAttrString(o, "grad");   // (a subclass may have its own)
+            if (!g) { Py_DECREF(grads); return nullptr; }
+            missing += g == Py_None;
+            PyList_SET_ITEM(grads, i, g);
+        }
+    } catch (const std::exception& e) {
+        Py_DECREF(grads);
+        PyErr_SetString(PyExc_ValueError, e.what());
+        return nullptr;
+    }
+    return Py_BuildValue("KNn", (unsigned long long)h, grads, missing);
 }
 
 // opt_table(what, params or None, grads, table, any_device) -> (entries, dtype code, length of the state buffers, gradients to reorder)
@@ -469,6 +494,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 }
 
 PyMethodDef kMethods[] = {{"opt_order", opt_order, METH_O, "a hash of sizes and strides"},
+                          {"opt_grads", opt_grads, METH_O, "that hash and the parameters' gradients"},
                           {"opt_table", opt_table, METH_VARARGS, "checks lists of tensors and writes their InsmosOptTensor table"},
                           {"bind_linear", bind_linear, METH_VARARGS, "addresses of the library's functions"},
                           {"linear", (PyCFunction)(void (*)())linear, METH_FASTCALL, "the layer, on the autograd tape"},

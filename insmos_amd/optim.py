@@ -203,10 +203,10 @@ class _Bucket:
         return out
 
 
-    def shares(self, grads):
+    def shares(self, grads, missing):
         """[(counter, gradients of its parameters)] for the parameters that have a gradient, and which parameters' counter has changed: where only some
-        of a counter's parameters have one, the others go on with a copy of it."""
-        if len(self.steps) == 1 and type(None) not in set(map(type, grads)):    # (the usual step: 4 us for 250 tensors)
+        of a counter's parameters have one, the others go on with a copy of it.  missing: how many have none."""
+        if len(self.steps) == 1 and not missing:     # (the usual step)
             return [(self.steps[0], grads)], []
         lists, moved = [], []
         for k in range(len(self.steps)):
@@ -282,9 +282,10 @@ class AdamW(torch.optim.Optimizer):
         work = []
         for gi, group in enumerate(self.param_groups):
             for b in self._group_buckets(gi):
-                if _host.opt_order(b.params) != b.order:
+                order, grads, missing = _host.opt_grads(b.params)
+                if order != b.order:
                     raise RuntimeError("AdamW: a parameter's shape or order in memory has changed since its state was made")
-                lists, moved = b.shares([p.grad for p in b.params])
+                lists, moved = b.shares(grads, missing)
                 for i in moved:
                     self.state[b.params[i]]["step"] = b.steps[b.counter[i]]
                 work += [(group, b, counter, grads) for counter, grads in lists]
