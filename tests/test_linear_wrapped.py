@@ -143,3 +143,20 @@ def test_linear_keeps_plain_subclasses():
     x, w, b, r = _layer()
     y = linear(x.as_subclass(_Marked), w, b, r, activation="gelu")
     assert type(y) is _Marked and torch.equal(y.as_subclass(torch.Tensor), linear(x, w, b, r, activation="gelu"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("out_in", [False, True])
+@pytest.mark.parametrize("act,first", [(0, False), (1, True), (1, False), (2, True), (4, False)])
+def test_linear_operator_is_registered_soundly(act, first, out_in, dtype):
+    """torch's own checks of the registered operators: schema (nothing mutated or aliased), autograd, fake results like the real ones."""
+    from insmos_amd import autograd as A
+    t = getattr(torch, dtype)
+    x, w, b, r = (v.to(t) for v in _layer())
+    w = w.t().contiguous().t() if out_in else w
+    leaves = [v.detach().requires_grad_() for v in (x, w, b, r)]
+    torch.library.opcheck(A._linear_op, (*leaves, act, first), test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))
+    y, slope = A._linear_op(x, w, b, r, act, first)
+    held = slope if act > 1 or not first else y
+    torch.library.opcheck(A._linear_backward_op, (torch.randn_like(y), held, x, w, act, not first, [True] * 4), test_utils=("test_schema", "test_faketensor"))
